@@ -50,8 +50,16 @@ class GemmTestcase(C.Structure):
     ]
 
 
+class Route(C.Structure):
+    """``tnns_route_t`` of include/tnns_b200.h."""
+    _fields_ = [(n, C.c_int) for n in ("experts", "top_k", "score", "groups", "top_groups", "group_top", "renormalise")] + [("scale", C.c_float)]
+
+    def __init__(self, experts, top_k, score=0, groups=1, top_groups=None, group_top=1, renormalise=1, scale=1.0):
+        super().__init__(experts, top_k, score, groups, groups if top_groups is None else top_groups, group_top, int(renormalise), scale)
+
+
 # name -> (restype, argtypes); every symbol include/tnns_b200.h declares
-_vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_vp, _i, _f, _sz, _ll = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_longlong
 _pf, _pi64 = C.POINTER(C.c_float), C.POINTER(C.c_int64)
 _pshape = C.POINTER(Shape)
 SHARD_FN = C.CFUNCTYPE(C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p)  # tnns_shard_fn
@@ -138,6 +146,14 @@ SIGNATURES = {
     "tnns_cuda_gemm_im2col_packed_out": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, C.c_float, _i, _vp]),
     "tnns_cuda_memcpy_h2d": (_i, [_vp, _vp, _vp, _sz]),
     "tnns_cuda_memcpy_d2h": (_i, [_vp, _vp, _vp, _sz]),
+    "tnns_cuda_quantise_i8": (_i, [_vp, _vp, _i, _ll, _vp, _ll, _vp, _i, _i, _vp]),
+    "tnns_cuda_upload_weights_i8": (_i, [_vp, _vp, _vp, _i, _i, _i, C.POINTER(_vp)]),
+    "tnns_cuda_free_weights_i8": (None, [_vp, _vp]),
+    "tnns_cuda_gemm_i8": (_i, [_vp, _vp, _vp, _ll, _vp, _vp, _i, _ll, _i, _f, _vp]),
+    "tnns_route_workspace_bytes": (_sz, [C.POINTER(Route), _i]),
+    "tnns_cuda_route": (_i, [_vp, C.POINTER(Route), _vp, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tnns_cuda_gemm_i8_experts": (_i, [_vp, _vp, _vp, _ll, _vp, _i, _vp, _vp, _vp, _i, _ll, _i, _f, _vp]),
+    "tnns_cuda_combine": (_i, [_vp, _vp, _i, _ll, _i, _vp, _vp, _i, _vp, _i, _ll, _i, _i, _vp]),
     "tnns_cuda_launch_count": (C.c_ulonglong, []),
     "tnns_cuda_last_error": (_i, []),
     "tnns_cuda_strerror": (C.c_char_p, [_i]),

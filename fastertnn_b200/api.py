@@ -12,12 +12,15 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import GemmTestcase, Shape, Testcase, load_library
+from ._lib import GemmTestcase, Route, Shape, Testcase, load_library
 
 TNN, TBN, BTN, BNN = 0, 1, 2, 3
 NCHW, NHWC = 0, 1
 PACK_AUTO, PACK_GATHER, PACK_STAGED = 0, 1, 2
 GEMM_AUTO, GEMM_POPC_SIMPLE, GEMM_POPC_TILED, GEMM_I8_TC, GEMM_F4_TC, GEMM_F4_FUSED, GEMM_F4_SLAB, GEMM_F4_SLAB_FUSED, GEMM_F4_DENSE = 0, 1, 2, 3, 4, 5, 6, 7, 8
+
+F32, F16, BF16 = 0, 1, 2
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 
 class TnnsError(RuntimeError):
@@ -225,6 +228,18 @@ class Weights:
             self.handle = None
 
 
+class WeightsI8:
+    """Device copy of the 8-bit weights of one layer (or of its experts)."""
+
+    def __init__(self, ctx: "Context", handle: int, experts: int, N: int, K: int):
+        self.ctx, self.handle, self.experts, self.N, self.K = ctx, handle, experts, N, K
+
+    def free(self):
+        if self.handle:
+            load_library().tnns_cuda_free_weights_i8(self.ctx.handle, self.handle)
+            self.handle = None
+
+
 class Context:
     """One ``tnns_cuda_ctx`` (per host thread and device)."""
 
@@ -415,6 +430,42 @@ class Context:
         """Host-pointer layer (addresses of pinned or pageable buffers)."""
         _check(self.lib.tnns_cuda_conv_host(self.handle, w.handle, h_x, h_thr, h_y, C.byref(shape), alpha, layout))
 
+    # -- products in 8-bit integers, routing to experts (strides in elements; 0: rows without gaps, 8-bit rows at the
+    #    next multiple of 16)
+    def upload_weights_i8(self, w: int, scales: int, N: int, K: int, experts: int = 1) -> WeightsI8:
+        """int8 [experts][N][K] and fp32 [experts][N] at host or device addresses."""
+        h = C.c_void_p()
+        _check(self.lib.tnns_cuda_upload_weights_i8(self.handle, w, scales, experts, N, K, C.byref(h)))
+        return WeightsI8(self, h.value, experts, N, K)
+
+    def quantise_i8(self, d_x: int, dtype: int, d_q: int, d_scale: int, M: int, K: int, x_stride=0, q_stride=0, stream=0):
+        """Rows of floats -> rows of 8-bit integers and one scale for each row."""
+        _check(self.lib.tnns_cuda_quantise_i8(self.handle, d_x, dtype, x_stride or K, d_q, q_stride or i8_pitch(K), d_scale, M, K, stream))
+
+    def gemm_i8(self, w: WeightsI8, d_q: int, d_scale: int, d_y: int, dtype: int, M: int, alpha: float = 1.0, q_stride=0, y_stride=0, stream=0):
+        """Product of quantised rows with 8-bit weights, scales of row and channel, PReLU."""
+        _check(self.lib.tnns_cuda_gemm_i8(self.handle, w.handle, d_q, q_stride or i8_pitch(w.K), d_scale, d_y, dtype, y_stride or w.N, M, alpha,
+                                          stream))
+
+    def route(self, route: Route, d_logits: int, dtype: int, d_bias: int, T: int, d_experts: int, d_weights: int, d_offsets: int = 0, d_rows: int = 0,
+              d_slots: int = 0, d_ws: int = 0, ws_bytes: int = 0, stride=0, stream=0):
+        """Experts and weights of T tokens, and (unless d_offsets is 0) the pairs in the experts' order.
+        d_ws: route_workspace_bytes() bytes."""
+        _check(self.lib.tnns_cuda_route(self.handle, C.byref(route), d_logits, dtype, stride or route.experts, d_bias, T, d_experts, d_weights, d_offsets,
+                                        d_rows, d_slots, d_ws, ws_bytes, stream))
+
+    def gemm_i8_experts(self, w: WeightsI8, d_q: int, d_scale: int, d_rows: int, d_offsets: int, d_y: int, dtype: int, q_rows: int, places: int,
+                        alpha: float = 1.0, q_stride=0, y_stride=0, stream=0):
+        """gemm_i8 of every expert over its places; d_rows: the row of every place (0: place p is row p)."""
+        _check(self.lib.tnns_cuda_gemm_i8_experts(self.handle, w.handle, d_q, q_stride or i8_pitch(w.K), d_scale, q_rows, d_rows, d_offsets, d_y, dtype,
+                                                  y_stride or w.N, places, alpha, stream))
+
+    def combine(self, d_y: int, dtype: int, places: int, d_slots: int, d_weights: int, top_k: int, d_out: int, out_dtype: int, T: int, N: int,
+                y_stride=0, out_stride=0, stream=0):
+        """Weighted sum of the experts' results of every token."""
+        _check(self.lib.tnns_cuda_combine(self.handle, d_y, dtype, y_stride or N, places, d_slots, d_weights, top_k, d_out, out_dtype,
+                                          out_stride or N, T, N, stream))
+
     def pipe_rate(self, op: int) -> float:
         """Issue rate of LOP3 (0), POPC (1) or IADD (2) in 1e9 thread-instructions per second, or of an
         issue-bound tcgen05.mma loop, kind::i8 (3) or kind::mxf4 (4), in 1e9 operations (2*M*N*K) per second."""
@@ -548,6 +599,15 @@ def conv_noalloc(type_: int, d_packed_weights: int, d_x: int, d_thr: int, d_y: i
     """Whole layer on the current device without any allocation: the packed matrix goes to
     the library's built-in scratch array (see tnns_cuda_conv_noalloc in the header)."""
     _check(load_library().tnns_cuda_conv_noalloc(type_, d_packed_weights, d_x, d_thr, d_y, C.byref(shape), alpha, layout, stream))
+
+
+def i8_pitch(K: int) -> int:
+    """Bytes from one 8-bit row to the next where the caller names no other: K rounded up to 16."""
+    return (K + 15) // 16 * 16
+
+
+def route_workspace_bytes(route: Route, T: int) -> int:
+    return int(load_library().tnns_route_workspace_bytes(C.byref(route), T))
 
 
 def packed_image_bytes(ternary: bool, N: int, C_: int, H: int, W: int) -> int:

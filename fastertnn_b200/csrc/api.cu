@@ -87,6 +87,7 @@ static int enter(const tnns_cuda_ctx* ctx, const tnns_cuda_weights* w = nullptr)
         return tnns_fail(TNNS_ERR_INVALID, "weights live on device %d, context on %d", w->device, ctx->device);
     return TNNS_OK;
 }
+int tnns_enter(const tnns_cuda_ctx* ctx) { return enter(ctx); }
 #define TNNS_ENTER(...)                   \
     do {                                  \
         int rc__ = enter(__VA_ARGS__);    \

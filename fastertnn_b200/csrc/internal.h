@@ -77,6 +77,9 @@ void tnns_count_launch(void);
 
 int tnns_make_geom(const tnns_shape_t* s, TnnsGeom* g);
 
+// the context's device becomes the thread's current one (api.cu)
+int tnns_enter(const tnns_cuda_ctx* ctx);
+
 // kernel launchers (all asynchronous on `stream`)
 int tnns_launch_pack(tnns_cuda_ctx* ctx, bool ternary, const float* d_x, const float* d_thr, void* d_packed,
                      const TnnsGeom& g, int layout, int algo, cudaStream_t stream);

@@ -484,6 +484,85 @@ size_t tnns_cuda_noalloc_scratch_bytes(void);
 int tnns_cuda_conv_noalloc(int type, const int64_t* d_packed_weights, const float* d_x, const float* d_thr, float* d_y,
                            const tnns_shape_t* s, float alpha, int layout, void* stream);
 
+/* ---- Products in 8-bit integers, routing to experts ----------------------------------------
+ * The layers of a ternary or binary network that need more than two bits -- its entry and classifier
+ * layers, products with outlying channels -- in 8-bit integers with fp32 scales, and the same spread
+ * over experts (no reference counterpart).  One layer of experts is
+ *     route -> quantise_i8 -> gemm_i8_experts -> quantise_i8 -> gemm_i8_experts -> combine.
+ * All are asynchronous on `stream`, need no workspace but tnns_cuda_route's, keep nothing from one call
+ * for the next, may be captured into a graph, and may run at the same time as other calls of the same
+ * context on other streams.  Rows and strides are counted in elements (bytes for 8-bit rows). */
+enum tnns_dtype { TNNS_F32 = 0, TNNS_F16 = 1, TNNS_BF16 = 2 };
+
+/* Rows of floats -> rows of 8-bit integers and one scale for each row: with a the row's largest magnitude,
+ * d_scale = a / 127 and q_k = x_k * 127 / a, the quotient of the real numbers rounded to the nearest integer,
+ * ties to even (not that of a rounded reciprocal).  A row of zeros: scale 0, q 0.  A row that holds an infinity
+ * or a NaN: scale NaN, q 0, so that the row's products are NaN.  d_x: M rows of K, x_stride elements apart,
+ * of type `dtype`; d_q: rows q_stride bytes apart (a multiple of 16, at least K), 16-byte aligned; the bytes
+ * between K and q_stride are left as they were.  The same call makes 8-bit weights with a scale for each
+ * channel out of N x K floats. */
+int tnns_cuda_quantise_i8(tnns_cuda_ctx* ctx, const void* d_x, int dtype, long long x_stride, int8_t* d_q, long long q_stride,
+                          float* d_scale, int M, int K, void* stream);
+
+typedef struct tnns_cuda_weights_i8 tnns_cuda_weights_i8; /* device copy of the 8-bit weights of one layer */
+/* 8-bit weights of `experts` kernels (1: a plain layer), each N x K without gaps, and a scale for each of their
+ * experts * N channels, both in host or device memory -> the tiles the kernels read (N and K rounded up to 128).
+ * K at most 131071: every sum then fits 32 bits.  Synchronises the device.  Done once per layer. */
+int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float* scales, int experts, int N, int K,
+                                tnns_cuda_weights_i8** out);
+void tnns_cuda_free_weights_i8(tnns_cuda_ctx* ctx, tnns_cuda_weights_i8* w);
+
+/* y[m][n] = PReLU(d_scale[m] * scales[n] * sum_k q[m][k] * w[n][k]), PReLU(v) = v > 0 ? v : v * alpha (alpha 1: none).
+ * The sum is exact (32-bit integers), scales and PReLU are applied in fp32, and the result is rounded once to `dtype`.
+ * d_q: M rows of K bytes, q_stride apart (a multiple of 16, at least K), 16-byte aligned; bytes behind K are not used.
+ * d_y: M rows of N, y_stride elements apart; what lies between N and y_stride is left as it was.  The layer must
+ * hold one kernel (experts = 1). */
+int tnns_cuda_gemm_i8(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale,
+                      void* d_y, int dtype, long long y_stride, int M, float alpha, void* stream);
+
+/* Routing of T tokens to experts.  Scores: softmax over the token's logits, or the sigmoid of each. */
+enum tnns_score { TNNS_ROUTE_SOFTMAX = 0, TNNS_ROUTE_SIGMOID = 1 };
+typedef struct tnns_route {
+    int experts;     /* 1 .. 1024 */
+    int top_k;       /* 1 .. 32, at most the experts of top_groups groups */
+    int score;       /* tnns_score */
+    int groups;      /* experts fall into this many equal groups (1 .. 32) of neighbours .. */
+    int top_groups;  /* .. of which the best so many are searched (groups: all) */
+    int group_top;   /* a group's worth: 1 = its best key, 2 = the sum of its two best values of score + bias */
+    int renormalise; /* weights are divided by (their sum + 1e-20) */
+    float scale;     /* weights are multiplied by this */
+} tnns_route_t;
+/* Experts are ranked by key: the logit where d_bias is NULL, score + bias[expert] otherwise, as 64-bit arithmetic
+ * orders them; equal keys go to the lower expert, equal groups to the lower group.  The bias moves the choice only:
+ * weights are made of the scores.  An expert whose logit is -inf or NaN, or whose bias is, is never chosen for that
+ * token (+inf counts as the largest finite float); slots that find no expert hold expert -1 and weight 0.
+ *   d_logits  T rows of `experts` of type `dtype`, `stride` elements apart
+ *   d_experts T x top_k, best first          d_weights  T x top_k floats
+ * and, unless all three are NULL, the pairs (token, slot) in the order of their experts, tokens ascending within
+ * an expert:
+ *   d_offsets experts + 1: the places of expert e are d_offsets[e] .. d_offsets[e + 1] - 1
+ *   d_rows    T x top_k: the token at every place, -1 behind the last pair
+ *   d_slots   T x top_k: the place of every pair, -1 where it has no expert
+ * d_workspace: tnns_route_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0); calls that can
+ * overlap on the GPU need one each. */
+size_t tnns_route_workspace_bytes(const tnns_route_t* r, int T);
+int tnns_cuda_route(tnns_cuda_ctx* ctx, const tnns_route_t* r, const void* d_logits, int dtype, long long stride, const float* d_bias, int T,
+                    int32_t* d_experts, float* d_weights, int32_t* d_offsets, int32_t* d_rows, int32_t* d_slots, void* d_workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* tnns_cuda_gemm_i8 for every expert at once: place p of expert e (d_offsets as above, in device memory, clamped to
+ * [0, places]) is y[p] = PReLU(d_scale[r] * scales[e] * W[e] q[r]) with r = d_rows[p], or p where d_rows is NULL.
+ * d_q / d_scale hold q_rows rows; an index outside of them reads as a row of zeros.  Rows of d_y behind the last
+ * pair are left as they were. */
+int tnns_cuda_gemm_i8_experts(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale,
+                              int q_rows, const int32_t* d_rows, const int32_t* d_offsets, void* d_y, int dtype, long long y_stride, int places,
+                              float alpha, void* stream);
+
+/* out[t] = sum_j d_weights[t][j] * y[d_slots[t][j]] over the top_k slots of token t, j ascending, in fp32, rounded
+ * once; slots outside [0, places) are skipped (a token without any gets zeros). */
+int tnns_cuda_combine(tnns_cuda_ctx* ctx, const void* d_y, int dtype, long long y_stride, int places, const int32_t* d_slots,
+                      const float* d_weights, int top_k, void* d_out, int out_dtype, long long out_stride, int T, int N, void* stream);
+
 /* Blocks until all work submitted through ctx's own streams has finished and reports
  * any asynchronous error, including the on-device status word. */
 int tnns_cuda_sync(tnns_cuda_ctx* ctx);

@@ -4,6 +4,7 @@
 #include <new>
 
 #include "dtype.cuh"
+#include "gemm_tc_common.cuh"
 #include "internal.h"
 
 // Weights as the kernels read them: tiles of 128 channels x 128 elements of K, 16 KB each, [expert][channel tile][K tile], zeros
@@ -19,6 +20,7 @@ struct tnns_cuda_weights_i8 {
 namespace {
 
 constexpr int WT = 128, WT_BYTES = WT * WT;
+constexpr int MAX_EXPERTS = 1024;
 
 __global__ void __launch_bounds__(256) tile_weights_kernel(const int8_t* __restrict__ w, int8_t* __restrict__ img, int N, int K, int n_tiles, int k_tiles,
                                                            long long pieces) {
@@ -46,64 +48,555 @@ struct GemmI8Args {
     void* y;
     long long y_stride;
     int q_rows, places, experts, N, K, n_tiles, k_tiles;
+    int dtype, y_vec;  // result type; bytes that may be stored at once everywhere in y
     float alpha;
+    unsigned int* status;
 };
 
-constexpr int SB = 64;  // places and channels of a block
+// The places of an expert, [first, last).
+__device__ __forceinline__ int2 places_of(const GemmI8Args& p, int e) {
+    if (!p.offsets) return make_int2(0, p.places);
+    const int first = min(max(p.offsets[e], 0), p.places);
+    return make_int2(first, min(max(p.offsets[e + 1], first), p.places));
+}
+// Row of q that a place reads, -1: none (reads as zeros).
+__device__ __forceinline__ int row_of(const GemmI8Args& p, int place) {
+    const int r = p.rows ? p.rows[place] : place;
+    return r >= 0 && r < p.q_rows ? r : -1;
+}
+__device__ __forceinline__ float prelu(float v, float alpha) { return v * (v > 0 ? 1.0f : alpha); }
 
-// 64 places x 64 channels a block, 16 x 16 threads of 4 x 4 outputs, four products an instruction on the integer pipe.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_i8_simple_kernel(GemmI8Args p) {
-    __shared__ uint32_t s_q[SB][33], s_w[SB][33];
-    const int e = blockIdx.z, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    int first = 0, last = p.places;
-    if (p.offsets) {
-        first = min(max(p.offsets[e], 0), p.places);
-        last = min(max(p.offsets[e + 1], first), p.places);
+// How a launch's work is dealt out: blocks of TM places of every expert, in the experts' order.  s_first[e] = blocks of the experts
+// before e; called by the whole block, ends with a barrier.  Sums saturate (overlapping offsets are the caller's mistake).
+template <int TM>
+__device__ __forceinline__ void list_blocks(const GemmI8Args& p, int* s_first, int tid, int threads) {
+    for (int e = tid; e < p.experts; e += threads) {
+        const int2 r = places_of(p, e);
+        s_first[e + 1] = (int)(((long long)r.y - r.x + TM - 1) / TM);
     }
-    const int n0 = blockIdx.y * SB;
-    for (int m0 = first + blockIdx.x * SB; m0 < last; m0 += gridDim.x * SB) {
-        int acc[4][4] = {};
-        for (int kt = 0; kt < p.k_tiles; kt++) {
-            __syncthreads();
-            for (int i = tid; i < SB * 32; i += 256) {
-                const int r = i >> 5, c = i & 31, k = kt * WT + c * 4;
-                const int place = m0 + r;
-                int row = place < last ? (p.rows ? p.rows[place] : place) : -1;
-                if (row >= p.q_rows) row = -1;
-                uint32_t v = 0;
-                if (row >= 0)
-                    for (int j = 0; j < 4; j++)
-                        if (k + j < p.K) v |= (uint32_t)(uint8_t)p.q[(long long)row * p.q_stride + k + j] << (8 * j);
-                s_q[r][c] = v;
-                const int n = n0 + r;
-                const int8_t* tile = p.img + (((long long)e * p.n_tiles + n / WT) * p.k_tiles + kt) * WT_BYTES;
-                s_w[r][c] = *reinterpret_cast<const uint32_t*>(tile + (n % WT) * 128 + (((c >> 2) ^ (n & 7)) << 4) + (c & 3) * 4);
+    if (tid == 0) s_first[0] = 0;
+    __syncthreads();
+    if (tid < 32) {
+        int carry = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + tid;
+            unsigned v = e < p.experts ? (unsigned)s_first[e + 1] : 0u;
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+                if (tid >= d) v = min(v + o, 0x3FFFFFFFu);
             }
-            __syncthreads();
-            for (int c = 0; c < 32; c++)
-                for (int i = 0; i < 4; i++)
-                    for (int j = 0; j < 4; j++) acc[i][j] = __dp4a((int)s_q[ty + 16 * i][c], (int)s_w[tx + 16 * j][c], acc[i][j]);
-        }
-        for (int i = 0; i < 4; i++) {
-            const int place = m0 + ty + 16 * i;
-            if (place >= last) continue;
-            const int row = p.rows ? p.rows[place] : place;
-            const float s = row >= 0 && row < p.q_rows ? p.scale[row] : 0.f;
-            for (int j = 0; j < 4; j++) {
-                const int n = n0 + tx + 16 * j;
-                if (n >= p.N) continue;
-                const float v = (float)acc[i][j] * s * p.w_scale[(long long)e * p.n_tiles * WT + n];
-                ((T*)p.y)[(long long)place * p.y_stride + n] = from_f32<T>(v > 0 ? v : v * p.alpha);
-            }
+            v = min(v + (unsigned)carry, 0x3FFFFFFFu);
+            if (e < p.experts) s_first[e + 1] = (int)v;
+            carry = (int)__shfl_sync(0xFFFFFFFFu, v, 31);
         }
     }
+    __syncthreads();
+}
+// The expert that block b belongs to: the last e with s_first[e] <= b.
+__device__ __forceinline__ int expert_of(const int* s_first, int experts, int b) {
+    int lo = 0, hi = experts;  // s_first[lo] <= b < s_first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_first[mid] <= b) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows: the weights are read once, straight into the operand registers of the warp-level matrix instruction
+// ---------------------------------------------------------------------------------------
+
+constexpr int FEW_WARPS = 8;
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 bytes of a row of q from byte k on; bytes behind K, which need not be readable, as zeros.
+__device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
+    if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int j = 0; k + j < K; j++) w[j >> 2] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 8*NT places x 16 channels a block, its warps taking the K tiles in turn and adding up their sums in shared memory.  Bounded by the
+// weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and g + 8, so four instructions multiply a whole K
+// tile of 2 KB and no byte passes through shared memory.  The order of K within the tile is the same for weights and rows.
+template <int NT>
+__global__ void __launch_bounds__(FEW_WARPS * 32) gemm_i8_few_kernel(GemmI8Args p) {
+    constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
+    extern __shared__ int s_first[];
+    __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    list_blocks<8 * NT>(p, s_first, tid, FEW_WARPS * 32);
+    const int n_blocks = (p.N + 15) / 16;
+    const long long items = (long long)s_first[p.experts] * n_blocks;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int b = (int)(item / n_blocks), n0 = (int)(item - (long long)b * n_blocks) * 16;
+        const int e = expert_of(s_first, p.experts, b);
+        const int2 range = places_of(p, e);
+        const int m0 = range.x + (b - s_first[e]) * 8 * NT;
+        const int8_t* wt = p.img + (((long long)e * p.n_tiles + n0 / WT) * p.k_tiles) * WT_BYTES + (n0 % WT + g) * 128;
+        const int8_t* row[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const int place = m0 + i * 8 + g, r = place < range.y ? row_of(p, place) : -1;
+            row[i] = r >= 0 ? p.q + (long long)r * p.q_stride : nullptr;
+        }
+        int acc[NT][4] = {};
+        for (int kt0 = warp; kt0 < p.k_tiles; kt0 += FEW_WARPS * U) {
+            uint4 a[U][4], x[U][NT][2];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int kt = kt0 + u * FEW_WARPS;
+                if (kt < p.k_tiles) {
+                    const int8_t* tile = wt + (long long)kt * WT_BYTES;
+                    a[u][0] = __ldg(reinterpret_cast<const uint4*>(tile + ((t ^ g) << 4)));
+                    a[u][1] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + ((t ^ g) << 4)));
+                    a[u][2] = __ldg(reinterpret_cast<const uint4*>(tile + (((t + 4) ^ g) << 4)));
+                    a[u][3] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + (((t + 4) ^ g) << 4)));
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int k = kt * WT + (t + 4 * h) * 16;
+                            x[u][i][h] = row[i] && k < p.K ? load_piece(row[i], k, p.K) : make_uint4(0, 0, 0, 0);
+                        }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (kt0 + u * FEW_WARPS < p.k_tiles) {
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        mma_s8(acc[i], a[u][0].x, a[u][1].x, a[u][2].x, a[u][3].x, x[u][i][0].x, x[u][i][1].x);
+                        mma_s8(acc[i], a[u][0].y, a[u][1].y, a[u][2].y, a[u][3].y, x[u][i][0].y, x[u][i][1].y);
+                        mma_s8(acc[i], a[u][0].z, a[u][1].z, a[u][2].z, a[u][3].z, x[u][i][0].z, x[u][i][1].z);
+                        mma_s8(acc[i], a[u][0].w, a[u][1].w, a[u][2].w, a[u][3].w, x[u][i][0].w, x[u][i][1].w);
+                    }
+                }
+        }
+        // d[0], d[1]: channel g, places 2t, 2t + 1; d[2], d[3]: channel g + 8
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s_sum[warp][i][(2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
+        __syncthreads();
+        for (int o = tid; o < NT * 128; o += FEW_WARPS * 32) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < FEW_WARPS; w++) sum += s_sum[w][o >> 7][o & 127];
+            const int place = m0 + (o >> 4), n = n0 + (o & 15);
+            if (place < range.y && n < p.N) {
+                const int r = row_of(p, place);
+                const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)e * p.n_tiles * WT + n], p.alpha);
+                const long long at = (long long)place * p.y_stride + n;
+                if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
+                else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
+                else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Many rows: 5th-generation tensor cores, accumulators in tensor memory
+// ---------------------------------------------------------------------------------------
+
+// Stages of 128 bytes of K: 128 rows of q (one tensor copy, or 32 gathers of four rows where places name their rows) and BN / CG
+// channels of weights (contiguous copies of the tiled image).
+template <int BN, int CG>
+struct TcI8 {
+    static constexpr int A_STAGE = BM * KCH, B_STAGE = BN / CG * KCH, STAGE = A_STAGE + B_STAGE;
+    static constexpr int NSTG = 200 * 1024 / STAGE;
+    static constexpr int NBUF = 2;  // accumulator sets
+    static constexpr int COLS = NBUF * BN < 32 ? 32 : NBUF * BN;
+    static constexpr int EPI0 = 4, EPI_WARPS = 8, THREADS = 32 * (EPI0 + EPI_WARPS);
+    static constexpr int BARS = 2 * NSTG + 2 * NBUF;
+    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + 4 * ((size_t)experts + 1); }
+};
+struct alignas(64) MapsI8 {
+    CUtensorMap q, w;
+};
+__device__ __forceinline__ void tc_mma_i8_lh(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %5, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_i8_pair_lh(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %5, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Four rows of a two-dimensional tensor, each 128 bytes from byte x on (the map's box is one row high).
+template <int CG>
+__device__ __forceinline__ void tma_gather4_g2s(uint32_t dst_smem, const void* tmap, int x, int4 r, uint32_t bar) {
+    if (CG == 2)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                     ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                     ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                     : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+          "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void store_32b(void* at, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// W words of a row at `at`, `vec` bytes at a time (32, 16, 8 or 4).
+template <int W>
+__device__ __forceinline__ void store_words(unsigned char* at, const uint32_t (&w)[W], int vec) {
+    if (vec >= 32) {
+#pragma unroll
+        for (int i = 0; i < W; i += 8) store_32b(at + 4 * i, w + i);
+    } else if (vec == 16) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else if (vec == 8) {
+#pragma unroll
+        for (int i = 0; i < W; i += 2) *reinterpret_cast<uint2*>(at + 4 * i) = make_uint2(w[i], w[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i++) *reinterpret_cast<uint32_t*>(at + 4 * i) = w[i];
+    }
+}
+// 32 neighbouring results of one row, of which the first `have` exist.
+__device__ __forceinline__ void store_results(const GemmI8Args& p, const float (&f)[32], long long at, int have) {
+    if (p.dtype == TNNS_F32) {
+        float* y = (float*)p.y + at;
+        if (have >= 32) {
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(f[j]);
+            store_words(reinterpret_cast<unsigned char*>(y), w, p.y_vec);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (j < have) y[j] = f[j];
+        }
+        return;
+    }
+    uint32_t w[16];
+    if (p.dtype == TNNS_F16) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    uint16_t* y = (uint16_t*)p.y + at;
+    if (have >= 32 && p.y_vec >= 4) {
+        store_words(reinterpret_cast<unsigned char*>(y), w, p.y_vec);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < have) y[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+    }
+}
+
+// All lanes of a warp wait; none leaves the loop before the others.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* status, unsigned code) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+
+// One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
+// of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
+// MMAs, warps 4 to 11 scale, round and store one accumulator while the MMAs fill the other.
+template <int BN, int CG>
+__global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(GemmI8Args p, const __grid_constant__ MapsI8 maps) {
+    using Cfg = TcI8<BN, CG>;
+    constexpr int NSTG = Cfg::NSTG, NBUF = Cfg::NBUF, TM = CG * BM;
+    // s32 accumulators, signed 8-bit operands, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+    constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char *sA = smem, *sB = smem + NSTG * Cfg::A_STAGE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + NSTG * Cfg::STAGE);
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * NSTG, bar_tfull = bar_empty + 8 * NSTG, bar_tempty = bar_tfull + 8 * NBUF;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* s_first = reinterpret_cast<int*>(tmem_slot + 4);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+    const int unit = blockIdx.x / CG, units = gridDim.x / CG;
+
+    if (tid == 0) {
+        for (int s = 0; s < NSTG; s++) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int b = 0; b < NBUF; b++) {
+            mbar_init(bar_tfull + 8 * b, 1);
+            mbar_init(bar_tempty + 8 * b, CG * Cfg::EPI_WARPS);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensor_map(&maps.q);
+        if (CG == 2) prefetch_tensor_map(&maps.w);
+    }
+    __syncwarp();
+    if (warp == WARP_MMA) {
+        if (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+    tc_fence_before();
+    if (CG == 2) cluster_sync_all(); else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // what follows reads and writes tensors that the launch in front may still be working on
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    list_blocks<TM>(p, s_first, tid, Cfg::THREADS);
+    const int n_blocks = (p.N + BN - 1) / BN;
+    const long long tiles = (long long)s_first[p.experts] * n_blocks;
+    struct Tile {
+        int e, m0, last, n;  // expert, first place, end of the expert's places, block of channels
+    };
+    // within an expert tiles run down RG row blocks before they move one block of channels on: what the SMs hold at one time is then
+    // about square, so that rows and weights both come out of L2
+    constexpr int RG = 8;
+    auto tile_at = [&](long long t) {
+        int b = (int)(t / n_blocks);
+        Tile r;
+        r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
+        const int2 range = places_of(p, r.e);
+        const int blocks = s_first[r.e + 1] - s_first[r.e];
+        const long long local = t - (long long)s_first[r.e] * n_blocks;
+        const int grp = (int)(local / ((long long)RG * n_blocks)), in = (int)(local - (long long)grp * RG * n_blocks);
+        const int high = min(RG, blocks - grp * RG);
+        r.n = in / high;
+        r.m0 = range.x + (grp * RG + in - r.n * high) * TM;
+        r.last = range.y;
+        return r;
+    };
+
+    if (warp == WARP_TMA) {
+        const uint32_t full_lead = CG == 2 ? mapa_shared(bar_full, 0) : bar_full;
+        uint32_t s = 0, ph = 1;
+        for (long long t = unit; t < tiles; t += units) {
+            const Tile c = tile_at(t);
+            const int m = c.m0 + (int)rank * BM;
+            int4 r = make_int4(0, 0, 0, 0);
+            if (p.rows) {  // lane: rows 4*lane .. + 3 of the block; what has no row takes row 0 and scale 0
+                int* ri = reinterpret_cast<int*>(&r);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int place = m + 4 * lane + i;
+                    ri[i] = place < c.last ? max(row_of(p, place), 0) : 0;
+                }
+            }
+            const int n0 = c.n * BN + (int)rank * (BN / CG);
+            for (int kt = 0; kt < p.k_tiles; kt++) {
+                if (!warp_wait(bar_empty + 8 * s, ph, abort_flag, p.status, 1)) goto done;
+                const uint32_t a_dst = smem_u32(sA + s * Cfg::A_STAGE), b_dst = smem_u32(sB + s * Cfg::B_STAGE), bar = full_lead + 8 * s;
+                if (lane == 0) {
+                    if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, CG * Cfg::STAGE);
+#pragma unroll
+                    for (int n = 0; n < BN / CG; n += WT) {
+                        constexpr int HIGH = BN / CG < WT ? BN / CG : WT;
+                        const int nn = n0 + n;
+                        // a tile of channels past the last repeats the last one: its results are not stored
+                        const long long tile = ((long long)c.e * p.n_tiles + min(nn / WT, p.n_tiles - 1)) * p.k_tiles + kt;
+                        if (CG == 2) tma_tile2d_g2s_pair(b_dst + n * KCH, &maps.w, 0, (int)(tile * WT + nn % WT), bar);
+                        else bulk_g2s(b_dst + n * KCH, p.img + tile * WT_BYTES + (nn % WT) * KCH, HIGH * KCH, bar);
+                    }
+                    if (!p.rows) {
+                        if (CG == 2) tma_tile2d_g2s_pair(a_dst, &maps.q, kt * KCH, m, bar);
+                        else tma_tile2d_g2s(a_dst, &maps.q, kt * KCH, m, bar);
+                    }
+                }
+                __syncwarp();
+                if (p.rows) tma_gather4_g2s<CG>(a_dst + lane * 512, &maps.q, kt * KCH, r, bar);
+                if (++s == NSTG) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == WARP_MMA) {
+        if (rank == 0) {
+            const bool elected = elect_one();
+            const uint64_t da0 = make_desc(smem_u32(sA)), db0 = make_desc(smem_u32(sB));
+            const uint32_t a_lo0 = (uint32_t)da0, a_hi = (uint32_t)(da0 >> 32), b_lo0 = (uint32_t)db0, b_hi = (uint32_t)(db0 >> 32);
+            uint32_t a_lo = a_lo0, b_lo = b_lo0, s = 0, ph = 0, lt = 0;
+            for (long long t = unit; t < tiles; t += units, lt++) {
+                const uint32_t buf = lt % NBUF;
+                if (!warp_wait(bar_tempty + 8 * buf, ((lt / NBUF) & 1) ^ 1, abort_flag, p.status, 2)) goto done;
+                tc_fence_after();
+                const uint32_t d = tmem_base + buf * BN;
+                for (int kt = 0; kt < p.k_tiles; kt++) {
+                    if (!warp_wait(bar_full + 8 * s, ph, abort_flag, p.status, 3)) goto done;
+                    tc_fence_after();
+                    if (elected) {
+#pragma unroll
+                        for (int k = 0; k < KCH / 32; k++) {
+                            if (CG == 2) tc_mma_i8_pair_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)(kt | k));
+                            else tc_mma_i8_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)(kt | k));
+                        }
+                        if (CG == 2) tc_commit_pair(bar_empty + 8 * s); else tc_commit(bar_empty + 8 * s);
+                    }
+                    if (++s == NSTG) { s = 0; ph ^= 1; a_lo = a_lo0; b_lo = b_lo0; }
+                    else { a_lo += Cfg::A_STAGE >> 4; b_lo += Cfg::B_STAGE >> 4; }
+                }
+                if (elected) {
+                    if (CG == 2) tc_commit_pair(bar_tfull + 8 * buf); else tc_commit(bar_tfull + 8 * buf);
+                }
+            }
+        }
+    } else if (warp >= Cfg::EPI0) {
+        const int q = warp & 3, half = (warp - Cfg::EPI0) >> 2;
+        const uint32_t tempty_lead = CG == 2 ? mapa_shared(bar_tempty, 0) : bar_tempty;
+        uint32_t lt = 0;
+        for (long long t = unit; t < tiles; t += units, lt++) {
+            const Tile c = tile_at(t);
+            const int place = c.m0 + (int)rank * BM + q * 32 + lane;
+            float rs = 0.f;
+            if (place < c.last) {
+                const int r = row_of(p, place);
+                if (r >= 0) rs = p.scale[r];
+            }
+            const uint32_t buf = lt % NBUF;
+            if (!warp_wait(bar_tfull + 8 * buf, (lt / NBUF) & 1, abort_flag, p.status, 4)) goto done;
+            tc_fence_after();
+            const float* ws = p.w_scale + (long long)c.e * p.n_tiles * WT;
+#pragma unroll 1
+            for (int cb = half * (BN / 2); cb < (half + 1) * (BN / 2); cb += 32) {
+                uint32_t v[32];
+                tmem_ld_32(tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + cb, v);
+                const int n = c.n * BN + cb;
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (cb + 32 == (half + 1) * (BN / 2)) {  // the last columns are in registers: the accumulator may be written again
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CG == 2) mbar_arrive_cluster(tempty_lead + 8 * buf); else mbar_arrive(bar_tempty + 8 * buf);
+                    }
+                }
+                if (n < p.N && place < c.last) {
+                    float f[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 w4 = __ldg(reinterpret_cast<const float4*>(ws + n + j));
+                        f[j] = prelu((float)(int)v[j] * rs * w4.x, p.alpha);
+                        f[j + 1] = prelu((float)(int)v[j + 1] * rs * w4.y, p.alpha);
+                        f[j + 2] = prelu((float)(int)v[j + 2] * rs * w4.z, p.alpha);
+                        f[j + 3] = prelu((float)(int)v[j + 3] * rs * w4.w, p.alpha);
+                    }
+                    store_results(p, f, (long long)place * p.y_stride + n, p.N - n);
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+done:
+    __syncwarp();
+    if (*abort_flag && warp == WARP_TMA && lane == 0) {
+        // a wait gave up: give the copies already requested time to land before shared memory is released
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
+    tc_fence_before();
+    if (CG == 2) cluster_sync_all(); else __syncthreads();
+    if (warp == WARP_MMA) {
+        tc_fence_after();
+        if (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::COLS) : "memory");
+    }
+}
+
+template <typename... Args>
+int launch(void (*kern)(Args...), tnns_cuda_ctx* ctx, int grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster;
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    TNNS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    tnns_count_launch();
+    TNNS_CUDA_TRY(cudaGetLastError());
+    return TNNS_OK;
+}
+
+template <int BN, int CG>
+int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
+    using Cfg = TcI8<BN, CG>;
+    MapsI8 maps = {};
+    // gathered rows: boxes of one row; else of the 128 rows of a block
+    int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, a.rows ? 1 : BM, 128);
+    if (rc) return rc;
+    // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
+    if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;
+    auto kern = gemm_i8_tc_kernel<BN, CG>;
+    static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
+    if (!smem_set[ctx->device & 63]) {
+        TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::smem(MAX_EXPERTS)));
+        smem_set[ctx->device & 63] = true;
+    }
+    const long long n_blocks = (a.N + BN - 1) / BN;
+    const long long most = ((long long)a.places + CG * BM - 1) / (CG * BM) + (a.offsets ? std::min(a.experts, a.places) : 0);
+    const int grid = CG * (int)std::min<long long>(most * n_blocks, ctx->sm_count / CG);
+    return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
+}
+
+template <int NT>
+int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
+    const long long n_blocks = (a.N + 15) / 16;
+    const long long most = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);
+    const int grid = (int)std::min<long long>(most * n_blocks, 8LL * ctx->sm_count);
+    return launch<GemmI8Args>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, 4 * ((size_t)a.experts + 1), 1, stream, a);
 }
 
 int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale, int q_rows,
                 const int32_t* d_rows, const int32_t* d_offsets, void* d_y, int dtype, long long y_stride, int places, float alpha, void* stream) {
     if (!tnns_dtype_ok(dtype)) return tnns_fail(TNNS_ERR_INVALID, "unknown element type %d", dtype);
-    if (places < 0 || q_rows < 0) return tnns_fail(TNNS_ERR_INVALID, "bad size: %d places, %d rows", places, q_rows);
+    if (places < 0 || places > 0x7FFFF000 || q_rows < 0) return tnns_fail(TNNS_ERR_INVALID, "bad size: %d places, %d rows", places, q_rows);
     if (q_stride < w->K || q_stride % 16 || y_stride < w->N)
         return tnns_fail(TNNS_ERR_INVALID, "rows of %d bytes at a stride of %lld (a multiple of 16), results of %d at %lld", w->K, q_stride, w->N, y_stride);
     if (places == 0) return TNNS_OK;
@@ -117,12 +610,19 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     a.img = w->d_img; a.w_scale = w->d_scale; a.q = d_q; a.q_stride = q_stride; a.scale = d_scale; a.rows = d_rows; a.offsets = d_offsets;
     a.y = d_y; a.y_stride = y_stride; a.q_rows = q_rows; a.places = places; a.experts = w->experts; a.N = w->N; a.K = w->K;
     a.n_tiles = w->n_tiles; a.k_tiles = w->k_tiles; a.alpha = alpha;
-    const dim3 grid(std::min((places + SB - 1) / SB, d_offsets ? 64 : 65535), (w->N + SB - 1) / SB, w->experts);
-    if (grid.y > 65535u || grid.z > 65535u) return tnns_fail(TNNS_ERR_UNSUPPORTED, "%d channels, %d experts", w->N, w->experts);
-    TNNS_FOR_DTYPE(dtype, T, (gemm_i8_simple_kernel<T><<<grid, 256, 0, (cudaStream_t)stream>>>(a)));
-    tnns_count_launch();
-    TNNS_CUDA_TRY(cudaGetLastError());
-    return TNNS_OK;
+    a.dtype = dtype; a.status = ctx->d_status;
+    const uintptr_t at = (uintptr_t)d_y | (uintptr_t)(y_stride * tnns_dtype_bytes(dtype));
+    a.y_vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : at % 8 == 0 ? 8 : at % 4 == 0 ? 4 : 2;
+    const cudaStream_t st = (cudaStream_t)stream;
+    // places an expert has on average
+    const long long rows = (long long)places / w->experts;
+    if (q_rows == 0 || rows <= 8) return launch_few<1>(ctx, a, st);
+    if (rows <= 16) return launch_few<2>(ctx, a, st);
+    if (rows <= 32) return launch_few<4>(ctx, a, st);
+    const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
+    if (tiles >= ctx->sm_count / 2) return launch_tc<256, 2>(ctx, a, st);
+    if (tiles * 4 >= ctx->sm_count) return launch_tc<128, 1>(ctx, a, st);
+    return launch_tc<64, 1>(ctx, a, st);
 }
 
 }  // namespace
@@ -133,7 +633,7 @@ int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float
                                 tnns_cuda_weights_i8** out) {
     if (!ctx || !w || !scales || !out) return tnns_fail(TNNS_ERR_INVALID, "NULL argument");
     *out = nullptr;
-    if (experts < 1 || experts > 65535 || N < 1 || K < 1 || K > 131071) return tnns_fail(TNNS_ERR_INVALID, "bad weight size: %d kernels of %d x %d (K at most 131071)", experts, N, K);
+    if (experts < 1 || experts > MAX_EXPERTS || N < 1 || K < 1 || K > 131071) return tnns_fail(TNNS_ERR_INVALID, "bad weight size: %d kernels (at most 1024) of %d x %d (K at most 131071)", experts, N, K);
     int rc = tnns_enter(ctx);
     if (rc) return rc;
     tnns_cuda_weights_i8* h = new (std::nothrow) tnns_cuda_weights_i8();

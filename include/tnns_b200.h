@@ -505,7 +505,7 @@ int tnns_cuda_quantise_i8(tnns_cuda_ctx* ctx, const void* d_x, int dtype, long l
                           float* d_scale, int M, int K, void* stream);
 
 typedef struct tnns_cuda_weights_i8 tnns_cuda_weights_i8; /* device copy of the 8-bit weights of one layer */
-/* 8-bit weights of `experts` kernels (1: a plain layer), each N x K without gaps, and a scale for each of their
+/* 8-bit weights of `experts` kernels (1: a plain layer; at most 1024), each N x K without gaps, and a scale for each of their
  * experts * N channels, both in host or device memory -> the tiles the kernels read (N and K rounded up to 128).
  * K at most 131071: every sum then fits 32 bits.  Synchronises the device.  Done once per layer. */
 int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float* scales, int experts, int N, int K,

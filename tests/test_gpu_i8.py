@@ -306,7 +306,8 @@ def expected_experts(q, scale, rows, offsets, w, w_scale, alpha, places):
 COUNTS = [
     ([1], 64, 32), ([0, 3, 0, 1], 100, 50), ([8] * 8, 256, 256), ([0] * 5 + [9], 130, 96), ([17, 0, 33, 5, 64], 512, 200), ([1, 2, 3, 0, 0, 7, 130], 300, 129),
     ([128, 129, 127, 1], 384, 256), ([300, 0, 12, 500], 640, 520), ([5] * 150, 96, 130), ([1000, 3, 1, 700], 1024, 264), ([2] * 300 + [0] * 20, 64, 70),
-    ([2000], 256, 513), ([40] * 30, 1100, 257), ([16] * 20 + [1], 777, 1000)]
+    ([2000], 256, 513), ([40] * 30, 1100, 257), ([16] * 20 + [1], 777, 1000), ([3000, 2500], 500, 1300),
+    ([700, 1, 900, 0, 257, 256, 255, 1400], 640, 2100)]
 
 
 @pytest.mark.parametrize("gather", [True, False])

@@ -207,15 +207,15 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) gemm_i8_few_kernel(GemmI8Args 
 // Many rows: 5th-generation tensor cores, accumulators in tensor memory
 // ---------------------------------------------------------------------------------------
 
-// Stages of 128 bytes of K: 128 rows of q (one tensor copy, or 32 gathers of four rows where places name their rows) and BN / CG
-// channels of weights (contiguous copies of the tiled image).
+// Stages of 128 bytes of K: 128 rows of q (one tensor copy, or 16-byte copies by the gather warps where places name their rows) and
+// BN / CG channels of weights (contiguous copies of the tiled image).
 template <int BN, int CG>
 struct TcI8 {
     static constexpr int A_STAGE = BM * KCH, B_STAGE = BN / CG * KCH, STAGE = A_STAGE + B_STAGE;
     static constexpr int NSTG = 200 * 1024 / STAGE;
     static constexpr int NBUF = 2;  // accumulator sets
     static constexpr int COLS = NBUF * BN < 32 ? 32 : NBUF * BN;
-    static constexpr int EPI0 = 4, EPI_WARPS = 8, THREADS = 32 * (EPI0 + EPI_WARPS);
+    static constexpr int GATHER0 = 2, GATHER_WARPS = 6, EPI0 = GATHER0 + GATHER_WARPS, EPI_WARPS = 8, THREADS = 32 * (EPI0 + EPI_WARPS);
     static constexpr int BARS = 2 * NSTG + 2 * NBUF;
     static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + 4 * ((size_t)experts + 1); }
 };
@@ -242,17 +242,9 @@ __device__ __forceinline__ void tc_mma_i8_pair_lh(uint32_t d_tmem, uint32_t a_lo
         ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Four rows of a two-dimensional tensor, each 128 bytes from byte x on (the map's box is one row high).
-template <int CG>
-__device__ __forceinline__ void tma_gather4_g2s(uint32_t dst_smem, const void* tmap, int x, int4 r, uint32_t bar) {
-    if (CG == 2)
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-                     ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-                     ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-                     : "memory");
+// 16 bytes from global to shared memory, of which the first `bytes` are fetched and the rest are zeros.
+__device__ __forceinline__ void copy16_async(uint32_t dst_smem, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
@@ -333,7 +325,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
 // of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
-// MMAs, warps 4 to 11 scale, round and store one accumulator while the MMAs fill the other.
+// MMAs, warps 2 to 7 gather rows where places name them (each a stage by itself, so six are on their way at once), warps 8 to 15
+// scale, round and store one accumulator while the MMAs fill the other.  Gathering through the copy engine, four rows a request,
+// was measured first: 80 clocks a request of 512 bytes, 360 us where the warps take X (8192 tokens, 8 of 64 experts, 2048 -> 1024).
 template <int BN, int CG>
 __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(GemmI8Args p, const __grid_constant__ MapsI8 maps) {
     using Cfg = TcI8<BN, CG>;
@@ -354,7 +348,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
 
     if (tid == 0) {
         for (int s = 0; s < NSTG; s++) {
-            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_full + 8 * s, p.rows ? 1 + CG : 1);  // the copies' bytes, and a gather warp of each block
             mbar_init(bar_empty + 8 * s, 1);
         }
         for (int b = 0; b < NBUF; b++) {
@@ -408,27 +402,18 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
         return r;
     };
 
+    const uint32_t full_lead = CG == 2 ? mapa_shared(bar_full, 0) : bar_full;
     if (warp == WARP_TMA) {
-        const uint32_t full_lead = CG == 2 ? mapa_shared(bar_full, 0) : bar_full;
-        uint32_t s = 0, ph = 1;
-        for (long long t = unit; t < tiles; t += units) {
-            const Tile c = tile_at(t);
-            const int m = c.m0 + (int)rank * BM;
-            int4 r = make_int4(0, 0, 0, 0);
-            if (p.rows) {  // lane: rows 4*lane .. + 3 of the block; what has no row takes row 0 and scale 0
-                int* ri = reinterpret_cast<int*>(&r);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int place = m + 4 * lane + i;
-                    ri[i] = place < c.last ? max(row_of(p, place), 0) : 0;
-                }
-            }
-            const int n0 = c.n * BN + (int)rank * (BN / CG);
-            for (int kt = 0; kt < p.k_tiles; kt++) {
-                if (!warp_wait(bar_empty + 8 * s, ph, abort_flag, p.status, 1)) goto done;
-                const uint32_t a_dst = smem_u32(sA + s * Cfg::A_STAGE), b_dst = smem_u32(sB + s * Cfg::B_STAGE), bar = full_lead + 8 * s;
-                if (lane == 0) {
-                    if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, CG * Cfg::STAGE);
+        if (lane == 0) {
+            const uint32_t bytes = CG * (p.rows ? Cfg::B_STAGE : Cfg::STAGE);
+            uint32_t s = 0, ph = 1;
+            for (long long t = unit; t < tiles; t += units) {
+                const Tile c = tile_at(t);
+                const int n0 = c.n * BN + (int)rank * (BN / CG), m = c.m0 + (int)rank * BM;
+                for (int kt = 0; kt < p.k_tiles; kt++) {
+                    if (!mbar_wait(bar_empty + 8 * s, ph, abort_flag, p.status, 1)) goto done;
+                    const uint32_t b_dst = smem_u32(sB + s * Cfg::B_STAGE), bar = full_lead + 8 * s;
+                    if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
 #pragma unroll
                     for (int n = 0; n < BN / CG; n += WT) {
                         constexpr int HIGH = BN / CG < WT ? BN / CG : WT;
@@ -439,13 +424,11 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
                         else bulk_g2s(b_dst + n * KCH, p.img + tile * WT_BYTES + (nn % WT) * KCH, HIGH * KCH, bar);
                     }
                     if (!p.rows) {
-                        if (CG == 2) tma_tile2d_g2s_pair(a_dst, &maps.q, kt * KCH, m, bar);
-                        else tma_tile2d_g2s(a_dst, &maps.q, kt * KCH, m, bar);
+                        if (CG == 2) tma_tile2d_g2s_pair(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
+                        else tma_tile2d_g2s(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
                     }
+                    if (++s == NSTG) { s = 0; ph ^= 1; }
                 }
-                __syncwarp();
-                if (p.rows) tma_gather4_g2s<CG>(a_dst + lane * 512, &maps.q, kt * KCH, r, bar);
-                if (++s == NSTG) { s = 0; ph ^= 1; }
             }
         }
     } else if (warp == WARP_MMA) {
@@ -478,7 +461,45 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
                 }
             }
         }
-    } else if (warp >= Cfg::EPI0) {
+    } else if (warp < Cfg::EPI0) {
+        if (p.rows) {
+            // stage i of the block's sequence belongs to gather warp i % 6
+            constexpr int GW = Cfg::GATHER_WARPS;
+            const int own = warp - Cfg::GATHER0;
+            uint32_t first = 0;  // stages of the tiles before this one, modulo GW and modulo 2 * NSTG
+            uint32_t slot0 = 0;
+            const uint32_t step = (uint32_t)p.k_tiles;
+            for (long long t = unit; t < tiles; t += units, first = (first + step) % GW, slot0 = (slot0 + step) % (2 * NSTG)) {
+                int kt = (own + GW - (int)first) % GW;
+                if (kt >= p.k_tiles) continue;
+                const Tile c = tile_at(t);
+                int r[4];  // rows lane, lane + 32, .. of the block's 128; -1: zeros
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int place = c.m0 + (int)rank * BM + 32 * i + lane;
+                    r[i] = place < c.last ? row_of(p, place) : -1;
+                }
+                for (; kt < p.k_tiles; kt += GW) {
+                    const uint32_t at = (slot0 + (uint32_t)kt) % (2 * NSTG), s = at % NSTG;
+                    if (!warp_wait(bar_empty + 8 * s, at < NSTG ? 1u : 0u, abort_flag, p.status, 5)) goto done;
+                    const int sub = lane >> 3, piece = lane & 7;  // of four rows an instruction: the row, and its 16-byte piece
+                    const int k = kt * KCH + piece * 16, have = min(max(p.K - k, 0), 16);
+                    const uint32_t a_dst = smem_u32(sA + s * Cfg::A_STAGE);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const int row = 4 * i + sub, src = __shfl_sync(0xFFFFFFFFu, r[i >> 3], row & 31);
+                        copy16_async(a_dst + row * KCH + ((piece ^ (row & 7)) << 4), p.q + (have ? (long long)max(src, 0) * p.q_stride + k : 0), src >= 0 ? have : 0);
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async();  // what this thread wrote, before the tensor core's reads
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CG == 2) mbar_arrive_cluster(full_lead + 8 * s); else mbar_arrive(bar_full + 8 * s);
+                    }
+                }
+            }
+        }
+    } else {
         const int q = warp & 3, half = (warp - Cfg::EPI0) >> 2;
         const uint32_t tempty_lead = CG == 2 ? mapa_shared(bar_tempty, 0) : bar_tempty;
         uint32_t lt = 0;
@@ -568,8 +589,7 @@ template <int BN, int CG>
 int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     using Cfg = TcI8<BN, CG>;
     MapsI8 maps = {};
-    // gathered rows: boxes of one row; else of the 128 rows of a block
-    int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, a.rows ? 1 : BM, 128);
+    int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, BM, 128);
     if (rc) return rc;
     // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
     if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;

@@ -150,8 +150,7 @@ SIGNATURES = {
     "tnns_cuda_upload_weights_i8": (_i, [_vp, _vp, _vp, _i, _i, _i, C.POINTER(_vp)]),
     "tnns_cuda_free_weights_i8": (None, [_vp, _vp]),
     "tnns_cuda_gemm_i8": (_i, [_vp, _vp, _vp, _ll, _vp, _vp, _i, _ll, _i, _f, _vp]),
-    "tnns_route_workspace_bytes": (_sz, [C.POINTER(Route), _i]),
-    "tnns_cuda_route": (_i, [_vp, C.POINTER(Route), _vp, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tnns_cuda_route": (_i, [_vp, C.POINTER(Route), _vp, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tnns_cuda_gemm_i8_experts": (_i, [_vp, _vp, _vp, _ll, _vp, _i, _vp, _vp, _vp, _i, _ll, _i, _f, _vp]),
     "tnns_cuda_combine": (_i, [_vp, _vp, _i, _ll, _i, _vp, _vp, _i, _vp, _i, _ll, _i, _i, _vp]),
     "tnns_cuda_launch_count": (C.c_ulonglong, []),

@@ -448,11 +448,10 @@ class Context:
                                           stream))
 
     def route(self, route: Route, d_logits: int, dtype: int, d_bias: int, T: int, d_experts: int, d_weights: int, d_offsets: int = 0, d_rows: int = 0,
-              d_slots: int = 0, d_ws: int = 0, ws_bytes: int = 0, stride=0, stream=0):
-        """Experts and weights of T tokens, and (unless d_offsets is 0) the pairs in the experts' order.
-        d_ws: route_workspace_bytes() bytes."""
+              d_slots: int = 0, stride=0, stream=0):
+        """Experts and weights of T tokens, and (unless d_offsets is 0) the pairs in the experts' order."""
         _check(self.lib.tnns_cuda_route(self.handle, C.byref(route), d_logits, dtype, stride or route.experts, d_bias, T, d_experts, d_weights, d_offsets,
-                                        d_rows, d_slots, d_ws, ws_bytes, stream))
+                                        d_rows, d_slots, stream))
 
     def gemm_i8_experts(self, w: WeightsI8, d_q: int, d_scale: int, d_rows: int, d_offsets: int, d_y: int, dtype: int, q_rows: int, places: int,
                         alpha: float = 1.0, q_stride=0, y_stride=0, stream=0):
@@ -604,10 +603,6 @@ def conv_noalloc(type_: int, d_packed_weights: int, d_x: int, d_thr: int, d_y: i
 def i8_pitch(K: int) -> int:
     """Bytes from one 8-bit row to the next where the caller names no other: K rounded up to 16."""
     return (K + 15) // 16 * 16
-
-
-def route_workspace_bytes(route: Route, T: int) -> int:
-    return int(load_library().tnns_route_workspace_bytes(C.byref(route), T))
 
 
 def packed_image_bytes(ternary: bool, N: int, C_: int, H: int, W: int) -> int:

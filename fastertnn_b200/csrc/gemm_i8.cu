@@ -120,64 +120,87 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 8*NT places x 16 channels a block, its warps taking the K tiles in turn and adding up their sums in shared memory.  Bounded by the
-// weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and g + 8, so four instructions multiply a whole K
-// tile of 2 KB and no byte passes through shared memory.  The order of K within the tile is the same for weights and rows.
+// 8 * NT places x 16 channels a warp, or S warps that share the K tiles and add up their sums in shared memory; a block holds 8 / S
+// such pieces side by side.  Bounded by the weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and
+// g + 8, so four instructions multiply a whole K tile of 2 KB and no byte passes through shared memory.  The order of K within the
+// tile is the same for weights and rows.
 template <int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32) gemm_i8_few_kernel(GemmI8Args p) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, NT == 4 ? 1 : 2) gemm_i8_few_kernel(GemmI8Args p, int S) {
     constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
     extern __shared__ int s_first[];
     __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int ks = warp & (S - 1), wide = FEW_WARPS / S * 16;  // this warp's part of K, channels of a block
+    const int n_blocks = (p.N + wide - 1) / wide;
+    const int8_t* wt;
+    uint4 a[U][4];
+    auto load_weights = [&](int kt0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (kt0 + u * S < p.k_tiles) {
+                const int8_t* tile = wt + (long long)(kt0 + u * S) * WT_BYTES;
+                a[u][0] = __ldg(reinterpret_cast<const uint4*>(tile + ((t ^ g) << 4)));
+                a[u][1] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + ((t ^ g) << 4)));
+                a[u][2] = __ldg(reinterpret_cast<const uint4*>(tile + (((t + 4) ^ g) << 4)));
+                a[u][3] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + (((t + 4) ^ g) << 4)));
+            }
+    };
+    auto weights_at = [&](int e, int n) { wt = p.img + ((long long)e * p.n_tiles + n / WT) * p.k_tiles * WT_BYTES + (n % WT + g) * 128; };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int n_mine = (warp / S) * 16;
+    bool loaded = false;
+    if (!p.offsets) {  // one kernel: the weights' way from memory may start before the launch in front has ended
+        const int n = (int)(blockIdx.x % (unsigned)n_blocks) * wide + n_mine;
+        if (n < p.N) {
+            weights_at(0, n);
+            load_weights(ks);
+        }
+        loaded = true;
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     list_blocks<8 * NT>(p, s_first, tid, FEW_WARPS * 32);
-    const int n_blocks = (p.N + 15) / 16;
     const long long items = (long long)s_first[p.experts] * n_blocks;
-    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-        const int b = (int)(item / n_blocks), n0 = (int)(item - (long long)b * n_blocks) * 16;
-        const int e = expert_of(s_first, p.experts, b);
+    for (long long item = blockIdx.x; item < items; item += gridDim.x, loaded = false) {
+        const int b = (int)(item / n_blocks), nb = (int)(item - (long long)b * n_blocks) * wide, n0 = nb + n_mine;
+        const int e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
+        int acc[NT][4] = {};
         const int2 range = places_of(p, e);
         const int m0 = range.x + (b - s_first[e]) * 8 * NT;
-        const int8_t* wt = p.img + (((long long)e * p.n_tiles + n0 / WT) * p.k_tiles) * WT_BYTES + (n0 % WT + g) * 128;
-        const int8_t* row[NT];
+        if (n0 < p.N) {
+            if (!loaded) {
+                weights_at(e, n0);
+                load_weights(ks);
+            }
+            const int8_t* row[NT];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const int place = m0 + i * 8 + g, r = place < range.y ? row_of(p, place) : -1;
-            row[i] = r >= 0 ? p.q + (long long)r * p.q_stride : nullptr;
-        }
-        int acc[NT][4] = {};
-        for (int kt0 = warp; kt0 < p.k_tiles; kt0 += FEW_WARPS * U) {
-            uint4 a[U][4], x[U][NT][2];
+            for (int i = 0; i < NT; i++) {
+                const int place = m0 + i * 8 + g, r = place < range.y ? row_of(p, place) : -1;
+                row[i] = r >= 0 ? p.q + (long long)r * p.q_stride : nullptr;
+            }
+            for (int kt0 = ks; kt0 < p.k_tiles; kt0 += S * U) {
+                uint4 x[U][NT][2];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int kt = kt0 + u * FEW_WARPS;
-                if (kt < p.k_tiles) {
-                    const int8_t* tile = wt + (long long)kt * WT_BYTES;
-                    a[u][0] = __ldg(reinterpret_cast<const uint4*>(tile + ((t ^ g) << 4)));
-                    a[u][1] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + ((t ^ g) << 4)));
-                    a[u][2] = __ldg(reinterpret_cast<const uint4*>(tile + (((t + 4) ^ g) << 4)));
-                    a[u][3] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + (((t + 4) ^ g) << 4)));
+                for (int u = 0; u < U; u++)
 #pragma unroll
                     for (int i = 0; i < NT; i++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int k = kt * WT + (t + 4 * h) * 16;
+                            const int k = (kt0 + u * S) * WT + (t + 4 * h) * 16;
                             x[u][i][h] = row[i] && k < p.K ? load_piece(row[i], k, p.K) : make_uint4(0, 0, 0, 0);
                         }
-                }
-            }
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (kt0 + u * FEW_WARPS < p.k_tiles) {
+                for (int u = 0; u < U; u++)
+                    if (kt0 + u * S < p.k_tiles) {
 #pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        mma_s8(acc[i], a[u][0].x, a[u][1].x, a[u][2].x, a[u][3].x, x[u][i][0].x, x[u][i][1].x);
-                        mma_s8(acc[i], a[u][0].y, a[u][1].y, a[u][2].y, a[u][3].y, x[u][i][0].y, x[u][i][1].y);
-                        mma_s8(acc[i], a[u][0].z, a[u][1].z, a[u][2].z, a[u][3].z, x[u][i][0].z, x[u][i][1].z);
-                        mma_s8(acc[i], a[u][0].w, a[u][1].w, a[u][2].w, a[u][3].w, x[u][i][0].w, x[u][i][1].w);
+                        for (int i = 0; i < NT; i++) {
+                            mma_s8(acc[i], a[u][0].x, a[u][1].x, a[u][2].x, a[u][3].x, x[u][i][0].x, x[u][i][1].x);
+                            mma_s8(acc[i], a[u][0].y, a[u][1].y, a[u][2].y, a[u][3].y, x[u][i][0].y, x[u][i][1].y);
+                            mma_s8(acc[i], a[u][0].z, a[u][1].z, a[u][2].z, a[u][3].z, x[u][i][0].z, x[u][i][1].z);
+                            mma_s8(acc[i], a[u][0].w, a[u][1].w, a[u][2].w, a[u][3].w, x[u][i][0].w, x[u][i][1].w);
+                        }
                     }
-                }
+                load_weights(kt0 + S * U);
+            }
         }
         // d[0], d[1]: channel g, places 2t, 2t + 1; d[2], d[3]: channel g + 8
 #pragma unroll
@@ -185,19 +208,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) gemm_i8_few_kernel(GemmI8Args 
 #pragma unroll
             for (int j = 0; j < 4; j++) s_sum[warp][i][(2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
         __syncthreads();
-        for (int o = tid; o < NT * 128; o += FEW_WARPS * 32) {
+        // a result for each place and channel of the block, channels side by side
+        for (int o = tid; o < 8 * NT * wide; o += FEW_WARPS * 32) {
+            const int c = o % wide, pl = o / wide, place = m0 + pl, n = nb + c;
+            if (place >= range.y || n >= p.N) continue;
             int sum = 0;
-#pragma unroll
-            for (int w = 0; w < FEW_WARPS; w++) sum += s_sum[w][o >> 7][o & 127];
-            const int place = m0 + (o >> 4), n = n0 + (o & 15);
-            if (place < range.y && n < p.N) {
-                const int r = row_of(p, place);
-                const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)e * p.n_tiles * WT + n], p.alpha);
-                const long long at = (long long)place * p.y_stride + n;
-                if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
-                else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
-                else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
-            }
+            for (int w = 0; w < S; w++) sum += s_sum[(c >> 4) * S + w][pl >> 3][(pl & 7) * 16 + (c & 15)];
+            const int r = row_of(p, place);
+            const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)e * p.n_tiles * WT + n], p.alpha);
+            const long long at = (long long)place * p.y_stride + n;
+            if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
+            else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
+            else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
         }
         __syncthreads();
     }
@@ -605,12 +627,16 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
 }
 
+// Warps that share the K tiles: at least four tiles a warp, so that their loads overlap, unless the pieces do not fill the SMs.
 template <int NT>
 int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
-    const long long n_blocks = (a.N + 15) / 16;
-    const long long most = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);
-    const int grid = (int)std::min<long long>(most * n_blocks, 8LL * ctx->sm_count);
-    return launch<GemmI8Args>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, 4 * ((size_t)a.experts + 1), 1, stream, a);
+    const long long high = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);  // at most
+    const long long pieces = high * ((a.N + 15) / 16);
+    int S = 1;
+    while (S < FEW_WARPS && S < a.k_tiles && (a.k_tiles >= 8 * S || pieces * S < 2LL * FEW_WARPS * ctx->sm_count)) S *= 2;
+    const int wide = FEW_WARPS / S * 16;
+    const int grid = (int)std::min<long long>(high * ((a.N + wide - 1) / wide), 8LL * ctx->sm_count);
+    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, 4 * ((size_t)a.experts + 1), 1, stream, a, S);
 }
 
 int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale, int q_rows,

@@ -110,33 +110,44 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits, float* scale) {
     if (scale) *scale = bad ? __int_as_float(0x7FC00000) : __fdiv_rn(r.a, 127.0f);
     return r;
 }
-// q = x * 127 / a of the real numbers, to the nearest integer, ties to even, for VE elements, as bytes.  r = x * fl(127 / a) is off
-// by at most two roundings of 2^-24 relative, 127 * 2^-23 < 2^-16 in all, so its nearest integer is the quotient's unless r lies
-// within 2^-15 of a half; there the quotient is formed in 64 bits, where x * 127 is exact (24 + 7 bits) and the division's one rounding
-// cannot reach a half that the quotient does not: they differ by 2^-32 relative or more.  Adding 1.5 * 2^23 rounds r to an
-// integer, ties to even, and leaves it in the low byte.
-template <int VE>
+// q = x * 127 / a of the real numbers, to the nearest integer, ties to even, for a chunk, as bytes.  r = x * fl(127 / a) is off by two
+// roundings, 2^-23 relative; adding 1.5 * 2^23 then rounds it to an integer, ties to even, and leaves that in the low byte.  What
+// remains is the quotient next to a half, h = n + 1/2:
+//   16-bit types  with x = X * 2^i, a = A * 2^j (X, A at most 11 bits) a quotient that is not h differs from it by
+//                 1 / max((2n + 1) * A, 127 * X) > 2^-19 relative.  So r, rounded to 21 bits, is h exactly where the quotient is,
+//                 and on the quotient's side of h where it is not: no case is left.
+//   fp32          where r lies within 2^-15 of a half, x * 127 and h * a are compared in 64 bits, where both are exact.
+// Rows whose largest magnitude is too small for 127 / a to be a float divide in 64 bits.
+template <typename T, int VE>
 __device__ __forceinline__ void quantise_chunk(const float (&x)[VE], const RowScale& s, uint32_t (&out)[VE / 4]) {
     constexpr float MAGIC = 12582912.0f;
     uint32_t q[VE];
-    float far = 0.f;
+    if (sizeof(T) == 2) {
 #pragma unroll
-    for (int j = 0; j < VE; j++) {
-        const float r = x[j] * s.inv, m = r + MAGIC;
-        far = fmaxf(far, fabsf(r - (m - MAGIC)));
-        q[j] = __float_as_uint(m);
-    }
-    if (far > 0.5f - 0x1p-15f || s.exact) {
-#pragma unroll 1
+        for (int j = 0; j < VE; j++) q[j] = __float_as_uint(__uint_as_float((__float_as_uint(x[j] * s.inv) + 4u) & ~7u) + MAGIC);
+    } else {
+        float far = 0.f;
+#pragma unroll
         for (int j = 0; j < VE; j++) {
-            // (indexing by a loop counter would send the registers to memory)
-            float v = x[0];
-#pragma unroll
-            for (int i = 1; i < VE; i++) v = i == j ? x[i] : v;
-            const uint32_t e = s.zero ? 0u : (uint32_t)(int)rint((double)v * 127.0 / (double)s.a);
-#pragma unroll
-            for (int i = 0; i < VE; i++) q[i] = i == j ? e : q[i];
+            const float r = x[j] * s.inv, m = r + MAGIC;
+            far = fmaxf(far, fabsf(r - (m - MAGIC)));
+            q[j] = __float_as_uint(m);
         }
+        if (far > 0.5f - 0x1p-15f) {
+#pragma unroll
+            for (int j = 0; j < VE; j++) {
+                const float r = fabsf(x[j] * s.inv), n = floorf(r);
+                if (fabsf(r - n - 0.5f) < 0x1p-15f) {
+                    const double d = (double)fabsf(x[j]) * 127.0 - ((double)n + 0.5) * (double)s.a;
+                    const int even = (int)n + ((int)n & 1), up = d > 0 ? (int)n + 1 : d < 0 ? (int)n : even;
+                    q[j] = (uint32_t)(x[j] < 0 ? -up : up);
+                }
+            }
+        }
+    }
+    if (s.exact) {
+#pragma unroll
+        for (int j = 0; j < VE; j++) q[j] = (uint32_t)(int)rint((double)x[j] * 127.0 / (double)s.a);
     }
 #pragma unroll
     for (int j = 0; j < VE / 4; j++) out[j] = s.zero ? 0u : __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
@@ -191,7 +202,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
         float f[VE];
         uint32_t w[VE / 4];
         unpack(ch, f);
-        quantise_chunk<VE>(f, s, w);
+        quantise_chunk<T, VE>(f, s, w);
         store_chunk<VE>(out, i, K, w);
     };
 #pragma unroll

@@ -489,7 +489,7 @@ int tnns_cuda_conv_noalloc(int type, const int64_t* d_packed_weights, const floa
  * layers, products with outlying channels -- in 8-bit integers with fp32 scales, and the same spread
  * over experts (no reference counterpart).  One layer of experts is
  *     route -> quantise_i8 -> gemm_i8_experts -> quantise_i8 -> gemm_i8_experts -> combine.
- * All are asynchronous on `stream`, need no workspace but tnns_cuda_route's, keep nothing from one call
+ * All are asynchronous on `stream`, need no workspace, keep nothing from one call
  * for the next, may be captured into a graph, and may run at the same time as other calls of the same
  * context on other streams.  Rows and strides are counted in elements (bytes for 8-bit rows). */
 enum tnns_dtype { TNNS_F32 = 0, TNNS_F16 = 1, TNNS_BF16 = 2 };
@@ -542,13 +542,9 @@ typedef struct tnns_route {
  * an expert:
  *   d_offsets experts + 1: the places of expert e are d_offsets[e] .. d_offsets[e + 1] - 1
  *   d_rows    T x top_k: the token at every place, -1 behind the last pair
- *   d_slots   T x top_k: the place of every pair, -1 where it has no expert
- * d_workspace: tnns_route_workspace_bytes() bytes, 16-byte aligned (NULL where that is 0); calls that can
- * overlap on the GPU need one each. */
-size_t tnns_route_workspace_bytes(const tnns_route_t* r, int T);
+ *   d_slots   T x top_k: the place of every pair, -1 where it has no expert */
 int tnns_cuda_route(tnns_cuda_ctx* ctx, const tnns_route_t* r, const void* d_logits, int dtype, long long stride, const float* d_bias, int T,
-                    int32_t* d_experts, float* d_weights, int32_t* d_offsets, int32_t* d_rows, int32_t* d_slots, void* d_workspace,
-                    size_t workspace_bytes, void* stream);
+                    int32_t* d_experts, float* d_weights, int32_t* d_offsets, int32_t* d_rows, int32_t* d_slots, void* stream);
 
 /* tnns_cuda_gemm_i8 for every expert at once: place p of expert e (d_offsets as above, in device memory, clamped to
  * [0, places]) is y[p] = PReLU(d_scale[r] * scales[e] * W[e] q[r]) with r = d_rows[p], or p where d_rows is NULL.

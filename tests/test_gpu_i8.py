@@ -439,15 +439,13 @@ class Layer:
         self.dx, self.dl, self.db = self.x.cuda(), self.logits.cuda(), self.bias.cuda()
         self.experts, self.weights, self.offsets = new(T, k, dtype=i32), new(T, k), new(E + 1, dtype=i32)
         self.rows, self.slots = new(P, dtype=i32), new(T, k, dtype=i32)
-        self.ws = new(max(16, ft.route_workspace_bytes(self.r, T)), dtype=torch.uint8)
         self.q1, self.sc1 = new(T, ft.i8_pitch(D), dtype=torch.int8), new(T)
         self.y1, self.q2, self.sc2 = new(P, H, dtype=torch.bfloat16), new(P, ft.i8_pitch(H), dtype=torch.int8), new(P)
         self.y2, self.out = new(P, D, dtype=torch.float32), new(T, D)
 
     def run(self, st):
         c, P, p = self.ctx, self.T * self.k, lambda t: t.data_ptr()
-        c.route(self.r, p(self.dl), ft.F32, p(self.db), self.T, p(self.experts), p(self.weights), p(self.offsets), p(self.rows), p(self.slots), p(self.ws),
-                self.ws.numel(), stream=st)
+        c.route(self.r, p(self.dl), ft.F32, p(self.db), self.T, p(self.experts), p(self.weights), p(self.offsets), p(self.rows), p(self.slots), stream=st)
         c.quantise_i8(p(self.dx), ft.BF16, p(self.q1), p(self.sc1), self.T, self.D, stream=st)
         c.gemm_i8_experts(self.h1, p(self.q1), p(self.sc1), p(self.rows), p(self.offsets), p(self.y1), ft.BF16, self.T, P, 0.5, stream=st)
         c.quantise_i8(p(self.y1), ft.BF16, p(self.q2), p(self.sc2), P, self.H, stream=st)

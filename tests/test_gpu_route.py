@@ -25,10 +25,9 @@ def run(ctx, r, logits, bias=None, with_plan=True, stride=None):
     i32 = torch.int32
     experts, weights = torch.full((T * r.top_k + 3,), -9, dtype=i32, device="cuda"), torch.full((T * r.top_k + 3,), -9.0, device="cuda")
     offsets, rows, slots = (torch.full((n + 3,), -9, dtype=i32, device="cuda") for n in (E + 1, T * r.top_k, T * r.top_k))
-    ws = torch.randint(0, 256, (max(16, ft.route_workspace_bytes(r, T)),), dtype=torch.uint8, device="cuda")
     for _ in range(2):
         ctx.route(r, view.data_ptr(), CODE[[n for n in DT if DT[n] == logits.dtype][0]], 0 if db is None else db.data_ptr(), T, experts.data_ptr(), weights.data_ptr(),
-                  *([offsets.data_ptr(), rows.data_ptr(), slots.data_ptr()] if with_plan else [0, 0, 0]), ws.data_ptr(), ws.numel(), stride=stride,
+                  *([offsets.data_ptr(), rows.data_ptr(), slots.data_ptr()] if with_plan else [0, 0, 0]), stride=stride,
                   stream=torch.cuda.current_stream().cuda_stream)
     ctx.sync()
     for t in (experts, weights, offsets, rows, slots):

@@ -185,7 +185,6 @@ def prepare(case, seed):
             ft, _ = _framework()
             s["route"] = ft.Route(experts=E, top_k=k, score=ft.ROUTE_SIGMOID if case["score"] == "sigmoid" else ft.ROUTE_SOFTMAX, groups=case["groups"],
                                   top_groups=case["top_groups"], group_top=case["group_top"], renormalise=int(case["renormalise"]), scale=case["scale"])
-            s["ws"] = torch.empty(max(16, ft.route_workspace_bytes(s["route"], T)), dtype=torch.uint8, device="cuda")
     else:
         T, E, k, K, N = (case[n] for n in "TEkKN")
         liking = torch.randn(T, E, generator=g, device="cuda") + case["skew"] * torch.randn(E, generator=g, device="cuda")
@@ -220,8 +219,7 @@ def _run_own(s):
         return s["y"]
     if op == "route":
         ctx.route(s["route"], s["logits"].data_ptr(), dt, 0 if s["bias"] is None else s["bias"].data_ptr(), case["T"], s["experts"].data_ptr(),
-                  s["weights"].data_ptr(), s["offsets"].data_ptr(), s["rows"].data_ptr(), s["slots"].data_ptr(), s["ws"].data_ptr(), s["ws"].numel(),
-                  stream=stream)
+                  s["weights"].data_ptr(), s["offsets"].data_ptr(), s["rows"].data_ptr(), s["slots"].data_ptr(), stream=stream)
         return s["experts"], s["weights"], s["offsets"], s["rows"], s["slots"]
     up = case["form"] == "up"
     ctx.gemm_i8_experts(s["handle"], s["q"].data_ptr(), s["scale"].data_ptr(), s["rows"].data_ptr() if up else 0, s["offsets"].data_ptr(),

@@ -67,12 +67,15 @@ __device__ __forceinline__ int row_of(const GemmI8Args& p, int place) {
 __device__ __forceinline__ float prelu(float v, float alpha) { return v * (v > 0 ? 1.0f : alpha); }
 
 // How a launch's work is dealt out: blocks of TM places of every expert, in the experts' order.  s_first[e] = blocks of the experts
-// before e; called by the whole block, ends with a barrier.  Sums saturate (overlapping offsets are the caller's mistake).
+// before e, s_range[e] = the expert's places; called by the whole block, ends with a barrier.  Sums saturate at `limit` (overlapping
+// offsets are the caller's mistake), so that what is counted on from them stays an int.
+constexpr size_t list_bytes(int experts) { return 8 * (size_t)experts + 4 * ((size_t)experts + 1); }
 template <int TM>
-__device__ __forceinline__ void list_blocks(const GemmI8Args& p, int* s_first, int tid, int threads) {
+__device__ __forceinline__ void list_blocks(const GemmI8Args& p, int2* s_range, int* s_first, unsigned limit, int tid, int threads) {
     for (int e = tid; e < p.experts; e += threads) {
         const int2 r = places_of(p, e);
-        s_first[e + 1] = (int)(((long long)r.y - r.x + TM - 1) / TM);
+        s_range[e] = r;
+        s_first[e + 1] = (int)min((unsigned)(r.y - r.x) / TM + ((unsigned)(r.y - r.x) % TM != 0), limit);
     }
     if (tid == 0) s_first[0] = 0;
     __syncthreads();
@@ -83,9 +86,9 @@ __device__ __forceinline__ void list_blocks(const GemmI8Args& p, int* s_first, i
             unsigned v = e < p.experts ? (unsigned)s_first[e + 1] : 0u;
             for (int d = 1; d < 32; d <<= 1) {
                 const unsigned o = __shfl_up_sync(0xFFFFFFFFu, v, d);
-                if (tid >= d) v = min(v + o, 0x3FFFFFFFu);
+                if (tid >= d) v = min(v + o, limit);
             }
-            v = min(v + (unsigned)carry, 0x3FFFFFFFu);
+            v = min(v + (unsigned)carry, limit);
             if (e < p.experts) s_first[e + 1] = (int)v;
             carry = (int)__shfl_sync(0xFFFFFFFFu, v, 31);
         }
@@ -125,9 +128,10 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 // g + 8, so four instructions multiply a whole K tile of 2 KB and no byte passes through shared memory.  The order of K within the
 // tile is the same for weights and rows.
 template <int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32, NT == 4 ? 1 : 2) gemm_i8_few_kernel(GemmI8Args p, int S) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Args p, int S) {
     constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
-    extern __shared__ int s_first[];
+    extern __shared__ int2 s_range[];
+    int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int ks = warp & (S - 1), wide = FEW_WARPS / S * 16;  // this warp's part of K, channels of a block
@@ -158,13 +162,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, NT == 4 ? 1 : 2) gemm_i8_few_k
         loaded = true;
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    list_blocks<8 * NT>(p, s_first, tid, FEW_WARPS * 32);
-    const long long items = (long long)s_first[p.experts] * n_blocks;
-    for (long long item = blockIdx.x; item < items; item += gridDim.x, loaded = false) {
-        const int b = (int)(item / n_blocks), nb = (int)(item - (long long)b * n_blocks) * wide, n0 = nb + n_mine;
+    list_blocks<8 * NT>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, FEW_WARPS * 32);
+    const int items = s_first[p.experts] * n_blocks;
+    for (int item = blockIdx.x; item < items; item += gridDim.x, loaded = false) {
+        const int b = item / n_blocks, nb = (item - b * n_blocks) * wide, n0 = nb + n_mine;
         const int e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
         int acc[NT][4] = {};
-        const int2 range = places_of(p, e);
+        const int2 range = s_range[e];
         const int m0 = range.x + (b - s_first[e]) * 8 * NT;
         if (n0 < p.N) {
             if (!loaded) {
@@ -234,12 +238,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, NT == 4 ? 1 : 2) gemm_i8_few_k
 template <int BN, int CG>
 struct TcI8 {
     static constexpr int A_STAGE = BM * KCH, B_STAGE = BN / CG * KCH, STAGE = A_STAGE + B_STAGE;
-    static constexpr int NSTG = 200 * 1024 / STAGE;
+    static constexpr int NSTG = 5 * 32768 / STAGE;
     static constexpr int NBUF = 2;  // accumulator sets
     static constexpr int COLS = NBUF * BN < 32 ? 32 : NBUF * BN;
     static constexpr int GATHER0 = 2, GATHER_WARPS = 6, EPI0 = GATHER0 + GATHER_WARPS, EPI_WARPS = 8, THREADS = 32 * (EPI0 + EPI_WARPS);
     static constexpr int BARS = 2 * NSTG + 2 * NBUF;
-    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + 4 * ((size_t)experts + 1); }
+    static constexpr int STAGED = 32;  // words of a row of a warp's buffer for results on their way out
+    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + EPI_WARPS * (32 * STAGED + BN / 2) * 4 + list_bytes(experts); }
 };
 struct alignas(64) MapsI8 {
     CUtensorMap q, w;
@@ -278,65 +283,86 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void store_32b(void* at, const uint32_t* w) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
-                 "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-// W words of a row at `at`, `vec` bytes at a time (32, 16, 8 or 4).
-template <int W>
-__device__ __forceinline__ void store_words(unsigned char* at, const uint32_t (&w)[W], int vec) {
-    if (vec >= 32) {
+// A warp's results leave through a buffer of 32 rows x 128 bytes in shared memory, so that it writes whole lines along the rows of
+// y: the 16-byte pieces of a row lie in the pattern piece ^ (row % 8), which keeps both directions free of bank conflicts.
+__device__ __forceinline__ uint32_t* staged(uint32_t* stage, int row, int word) { return stage + row * 32 + ((((word >> 2) ^ row) & 7) << 2) + (word & 3); }
+
+// Rows 0 .. rows - 1 of the buffer to `y`, `step` bytes from row to row; `have` bytes of each exist (a multiple of `size`, an element's
+// bytes).  vec: bytes that may be stored at once everywhere in y.
+__device__ __forceinline__ void store_rows(uint32_t* stage, unsigned char* y, long long step, int rows, int have, int vec, int size, int lane) {
+    if (vec >= 16 && have % 16 == 0) {
+        unsigned char* at = y + (lane >> 3) * step + (lane & 7) * 16;
 #pragma unroll
-        for (int i = 0; i < W; i += 8) store_32b(at + 4 * i, w + i);
-    } else if (vec == 16) {
-#pragma unroll
-        for (int i = 0; i < W; i += 4) *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    } else if (vec == 8) {
-#pragma unroll
-        for (int i = 0; i < W; i += 2) *reinterpret_cast<uint2*>(at + 4 * i) = make_uint2(w[i], w[i + 1]);
+        for (int i = 0; i < 8; i++, at += 4 * step) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(staged(stage, r, 4 * (lane & 7)));
+            if (r < rows && 16 * (lane & 7) < have) *reinterpret_cast<uint4*>(at) = v;
+        }
     } else {
-#pragma unroll
-        for (int i = 0; i < W; i++) *reinterpret_cast<uint32_t*>(at + 4 * i) = w[i];
+        for (int r = 0; r < rows; r++, y += step) {
+            const uint32_t v = *staged(stage, r, lane);
+            if (size == 4 || (reinterpret_cast<uintptr_t>(y) & 2) == 0) {
+                if (4 * lane + 4 <= have) *reinterpret_cast<uint32_t*>(y + 4 * lane) = v;
+                else if (4 * lane + 2 <= have) *reinterpret_cast<uint16_t*>(y + 4 * lane) = (uint16_t)v;
+            } else {
+                // a row that starts between two words: the halves of neighbours together, the first and the last by themselves
+                const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+                if (lane == 0) *reinterpret_cast<uint16_t*>(y) = (uint16_t)v;
+                if (4 * lane + 6 <= have) *reinterpret_cast<uint32_t*>(y + 2 + 4 * lane) = __funnelshift_r(v, next, 16);
+                else if (4 * lane + 4 <= have) *reinterpret_cast<uint16_t*>(y + 2 + 4 * lane) = (uint16_t)(v >> 16);
+            }
+        }
     }
 }
-// 32 neighbouring results of one row, of which the first `have` exist.
-__device__ __forceinline__ void store_results(const GemmI8Args& p, const float (&f)[32], long long at, int have) {
-    if (p.dtype == TNNS_F32) {
-        float* y = (float*)p.y + at;
-        if (have >= 32) {
-            uint32_t w[32];
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+// Two neighbouring results of a row: the row's scale, the channels' scales, PReLU (slope between 0 and 1: the larger of v and
+// alpha * v; mode 0: none, 1: that, 2: any slope).
+__device__ __forceinline__ float2 finish_pair(uint32_t a0, uint32_t a1, float rs, float2 ws, float alpha, int mode) {
+    float2 f = mul2(mul2(make_float2((float)(int)a0, (float)(int)a1), make_float2(rs, rs)), ws);
+    if (mode == 1) {
+        const float2 g = mul2(f, make_float2(alpha, alpha));
+        f = make_float2(fmaxf(f.x, g.x), fmaxf(f.y, g.y));
+    } else if (mode == 2) {
+        f = make_float2(prelu(f.x, alpha), prelu(f.y, alpha));
+    }
+    return f;
+}
+// 32 accumulators of the lane's row -> bytes of the buffer's row from word w0 on.
+__device__ __forceinline__ void finish_chunk(int dtype, const uint32_t (&v)[32], float rs, const float* ws, float alpha, int mode, uint32_t* stage, int lane, int w0) {
+    if (dtype == TNNS_F32) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) w[j] = __float_as_uint(f[j]);
-            store_words(reinterpret_cast<unsigned char*>(y), w, p.y_vec);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; j++)
-                if (j < have) y[j] = f[j];
+        for (int j = 0; j < 32; j += 4) {
+            const float4 w4 = *reinterpret_cast<const float4*>(ws + j);
+            const float2 a = finish_pair(v[j], v[j + 1], rs, make_float2(w4.x, w4.y), alpha, mode), b = finish_pair(v[j + 2], v[j + 3], rs, make_float2(w4.z, w4.w), alpha, mode);
+            *reinterpret_cast<float4*>(staged(stage, lane, j)) = make_float4(a.x, a.y, b.x, b.y);
         }
         return;
     }
-    uint32_t w[16];
-    if (p.dtype == TNNS_F16) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int j = 0; j < 32; j += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const float4 w4 = *reinterpret_cast<const float4*>(ws + j + 2 * i);
+            const float2 a = finish_pair(v[j + 2 * i], v[j + 2 * i + 1], rs, make_float2(w4.x, w4.y), alpha, mode);
+            const float2 b = finish_pair(v[j + 2 * i + 2], v[j + 2 * i + 3], rs, make_float2(w4.z, w4.w), alpha, mode);
+            if (dtype == TNNS_F16) {
+                const __half2 x = __floats2half2_rn(a.x, a.y), y = __floats2half2_rn(b.x, b.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+                w[i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+            } else {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a.x, a.y), y = __floats2bfloat162_rn(b.x, b.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+                w[i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+            }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
-    uint16_t* y = (uint16_t*)p.y + at;
-    if (have >= 32 && p.y_vec >= 4) {
-        store_words(reinterpret_cast<unsigned char*>(y), w, p.y_vec);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (j < have) y[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+        *reinterpret_cast<uint4*>(staged(stage, lane, w0 + (j >> 1))) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -347,7 +373,7 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
 // of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
-// MMAs, warps 2 to 7 gather rows where places name them (each a stage by itself, so six are on their way at once), warps 8 to 15
+// MMAs, warps 2 to 7 gather rows where places name them (each a slot of the ring, so that all are on their way at once), warps 8 to 15
 // scale, round and store one accumulator while the MMAs fill the other.  Gathering through the copy engine, four rows a request,
 // was measured first: 80 clocks a request of 512 bytes, 360 us where the warps take X (8192 tokens, 8 of 64 experts, 2048 -> 1024).
 template <int BN, int CG>
@@ -363,7 +389,10 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * NSTG, bar_tfull = bar_empty + 8 * NSTG, bar_tempty = bar_tfull + 8 * NBUF;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* s_first = reinterpret_cast<int*>(tmem_slot + 4);
+    uint32_t* s_stage = tmem_slot + 4;                                                      // [epilogue warp][32][STAGED]
+    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][BN / 2]: its channels' scales
+    int2* s_range = reinterpret_cast<int2*>(s_ws + Cfg::EPI_WARPS * (BN / 2));
+    int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
     const int unit = blockIdx.x / CG, units = gridDim.x / CG;
@@ -400,23 +429,22 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
 
     // what follows reads and writes tensors that the launch in front may still be working on
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    list_blocks<TM>(p, s_first, tid, Cfg::THREADS);
     const int n_blocks = (p.N + BN - 1) / BN;
-    const long long tiles = (long long)s_first[p.experts] * n_blocks;
+    list_blocks<TM>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, Cfg::THREADS);
+    const int tiles = s_first[p.experts] * n_blocks;
     struct Tile {
         int e, m0, last, n;  // expert, first place, end of the expert's places, block of channels
     };
     // within an expert tiles run down RG row blocks before they move one block of channels on: what the SMs hold at one time is then
     // about square, so that rows and weights both come out of L2
     constexpr int RG = 8;
-    auto tile_at = [&](long long t) {
-        int b = (int)(t / n_blocks);
+    auto tile_at = [&](int t) {
+        const int b = t / n_blocks;
         Tile r;
         r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
-        const int2 range = places_of(p, r.e);
-        const int blocks = s_first[r.e + 1] - s_first[r.e];
-        const long long local = t - (long long)s_first[r.e] * n_blocks;
-        const int grp = (int)(local / ((long long)RG * n_blocks)), in = (int)(local - (long long)grp * RG * n_blocks);
+        const int2 range = s_range[r.e];
+        const int before = s_first[r.e], blocks = s_first[r.e + 1] - before, local = t - before * n_blocks;
+        const int grp = (b - before) / RG, in = local - grp * RG * n_blocks;
         const int high = min(RG, blocks - grp * RG);
         r.n = in / high;
         r.m0 = range.x + (grp * RG + in - r.n * high) * TM;
@@ -429,7 +457,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
         if (lane == 0) {
             const uint32_t bytes = CG * (p.rows ? Cfg::B_STAGE : Cfg::STAGE);
             uint32_t s = 0, ph = 1;
-            for (long long t = unit; t < tiles; t += units) {
+            for (int t = unit; t < tiles; t += units) {
                 const Tile c = tile_at(t);
                 const int n0 = c.n * BN + (int)rank * (BN / CG), m = c.m0 + (int)rank * BM;
                 for (int kt = 0; kt < p.k_tiles; kt++) {
@@ -459,7 +487,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
             const uint64_t da0 = make_desc(smem_u32(sA)), db0 = make_desc(smem_u32(sB));
             const uint32_t a_lo0 = (uint32_t)da0, a_hi = (uint32_t)(da0 >> 32), b_lo0 = (uint32_t)db0, b_hi = (uint32_t)(db0 >> 32);
             uint32_t a_lo = a_lo0, b_lo = b_lo0, s = 0, ph = 0, lt = 0;
-            for (long long t = unit; t < tiles; t += units, lt++) {
+            for (int t = unit; t < tiles; t += units, lt++) {
                 const uint32_t buf = lt % NBUF;
                 if (!warp_wait(bar_tempty + 8 * buf, ((lt / NBUF) & 1) ^ 1, abort_flag, p.status, 2)) goto done;
                 tc_fence_after();
@@ -485,15 +513,18 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
         }
     } else if (warp < Cfg::EPI0) {
         if (p.rows) {
-            // stage i of the block's sequence belongs to gather warp i % 6
-            constexpr int GW = Cfg::GATHER_WARPS;
+            // Stage i of the block's sequence belongs to gather warp i % NSTG, and so does its slot of the ring: a warp's successive waits on a
+            // slot's barrier are then successive phases, which is all that a parity tells apart.  (Six warps on five slots met a slot again
+            // one lap early and wrote over a stage that was still to be read; the launch failed.)
+            constexpr int GW = NSTG;
+            static_assert(GW <= Cfg::GATHER_WARPS, "a gather warp for every slot");
             const int own = warp - Cfg::GATHER0;
             uint32_t first = 0;  // stages of the tiles before this one, modulo GW and modulo 2 * NSTG
             uint32_t slot0 = 0;
             const uint32_t step = (uint32_t)p.k_tiles;
-            for (long long t = unit; t < tiles; t += units, first = (first + step) % GW, slot0 = (slot0 + step) % (2 * NSTG)) {
+            for (int t = unit; t < tiles; t += units, first = (first + step) % GW, slot0 = (slot0 + step) % (2 * NSTG)) {
                 int kt = (own + GW - (int)first) % GW;
-                if (kt >= p.k_tiles) continue;
+                if (own >= GW || kt >= p.k_tiles) continue;
                 const Tile c = tile_at(t);
                 int r[4];  // rows lane, lane + 32, .. of the block's 128; -1: zeros
 #pragma unroll
@@ -523,46 +554,72 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
         }
     } else {
         const int q = warp & 3, half = (warp - Cfg::EPI0) >> 2;
+        constexpr int HN = BN / 2, NC = HN / 32;  // channels of the half, in chunks of 32
         const uint32_t tempty_lead = CG == 2 ? mapa_shared(bar_tempty, 0) : bar_tempty;
+        uint32_t* stage = s_stage + (warp - Cfg::EPI0) * 32 * Cfg::STAGED;
+        const int mode = p.alpha == 1.0f ? 0 : p.alpha > 0.0f && p.alpha < 1.0f ? 1 : 2;
+        // what a tile's results are scaled with is fetched while the tile before is on its way out
+        Tile c = {};
+        int row = -1;
+        float rs = 0.f, ws[NC];
+        float* wsc = s_ws + (warp - Cfg::EPI0) * HN;
+        auto fetch = [&](int t) {
+            c = tile_at(t);
+            const int place = c.m0 + (int)rank * BM + q * 32 + lane, n = c.n * BN + half * HN + lane;
+            row = place < c.last ? row_of(p, place) : -1;
+#pragma unroll
+            for (int i = 0; i < NC; i++) ws[i] = n + 32 * i < p.N ? __ldg(p.w_scale + (long long)c.e * p.n_tiles * WT + n + 32 * i) : 0.f;
+        };
+        if (unit < tiles) {
+            fetch(unit);
+            rs = row >= 0 ? p.scale[row] : 0.f;
+        }
         uint32_t lt = 0;
-        for (long long t = unit; t < tiles; t += units, lt++) {
-            const Tile c = tile_at(t);
-            const int place = c.m0 + (int)rank * BM + q * 32 + lane;
-            float rs = 0.f;
-            if (place < c.last) {
-                const int r = row_of(p, place);
-                if (r >= 0) rs = p.scale[r];
-            }
+        for (int t = unit; t < tiles; t += units, lt++) {
             const uint32_t buf = lt % NBUF;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < NC; i++) wsc[32 * i + lane] = ws[i];
+            __syncwarp();
+            const Tile now = c;
+            const float rs_now = rs;
+            const int place0 = now.m0 + (int)rank * BM + q * 32, rows_here = min(32, now.last - place0);
             if (!warp_wait(bar_tfull + 8 * buf, (lt / NBUF) & 1, abort_flag, p.status, 4)) goto done;
             tc_fence_after();
-            const float* ws = p.w_scale + (long long)c.e * p.n_tiles * WT;
-#pragma unroll 1
-            for (int cb = half * (BN / 2); cb < (half + 1) * (BN / 2); cb += 32) {
-                uint32_t v[32];
-                tmem_ld_32(tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + cb, v);
-                const int n = c.n * BN + cb;
+            if (t + units < tiles) fetch(t + units);
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + half * HN;
+            const int n0 = now.n * BN + half * HN, size = p.dtype == TNNS_F32 ? 4 : 2;
+            unsigned char* y0 = (unsigned char*)p.y + ((long long)place0 * p.y_stride + n0) * size;
+            const long long step = p.y_stride * size;
+            // a pass: as many channels as two loads of 32, and 128 bytes of every row (fp32: twice)
+            constexpr int CH = NC < 2 ? 1 : 2;
+#pragma unroll
+            for (int i = 0; i < NC; i += CH) {
+                uint32_t v[CH][32];
+#pragma unroll
+                for (int h = 0; h < CH; h++) tmem_ld_32(taddr + 32 * (i + h), v[h]);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (cb + 32 == (half + 1) * (BN / 2)) {  // the last columns are in registers: the accumulator may be written again
+                if (i + CH >= NC) {  // the last columns are in registers: the accumulator may be written again
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         if (CG == 2) mbar_arrive_cluster(tempty_lead + 8 * buf); else mbar_arrive(bar_tempty + 8 * buf);
                     }
                 }
-                if (n < p.N && place < c.last) {
-                    float f[32];
+                if (i == 0) rs = row >= 0 ? p.scale[row] : 0.f;  // the next tile's
+                if (rows_here > 0 && n0 + 32 * i < p.N) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 w4 = __ldg(reinterpret_cast<const float4*>(ws + n + j));
-                        f[j] = prelu((float)(int)v[j] * rs * w4.x, p.alpha);
-                        f[j + 1] = prelu((float)(int)v[j + 1] * rs * w4.y, p.alpha);
-                        f[j + 2] = prelu((float)(int)v[j + 2] * rs * w4.z, p.alpha);
-                        f[j + 3] = prelu((float)(int)v[j + 3] * rs * w4.w, p.alpha);
+                    for (int h = 0; h < CH; h++) {
+                        finish_chunk(p.dtype, v[h], rs_now, wsc + 32 * (i + h), p.alpha, mode, stage, lane, 16 * h);
+                        if (size == 4 || h + 1 == CH) {
+                            const int first = size == 4 ? i + h : i;  // of the chunks in the buffer
+                            const int have = min(p.N - n0 - 32 * first, size == 4 ? 32 : 32 * CH) * size;
+                            __syncwarp();
+                            if (have > 0) store_rows(stage, y0 + 32 * first * size, step, rows_here, have, p.y_vec, size, lane);
+                            __syncwarp();
+                        }
                     }
-                    store_results(p, f, (long long)place * p.y_stride + n, p.N - n);
                 }
-                __syncwarp();
             }
         }
     }
@@ -623,6 +680,7 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     }
     const long long n_blocks = (a.N + BN - 1) / BN;
     const long long most = ((long long)a.places + CG * BM - 1) / (CG * BM) + (a.offsets ? std::min(a.experts, a.places) : 0);
+    if (most * n_blocks >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many tiles: %d places of %d channels", a.places, a.N);
     const int grid = CG * (int)std::min<long long>(most * n_blocks, ctx->sm_count / CG);
     return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
 }
@@ -635,8 +693,10 @@ int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     int S = 1;
     while (S < FEW_WARPS && S < a.k_tiles && (a.k_tiles >= 8 * S || pieces * S < 2LL * FEW_WARPS * ctx->sm_count)) S *= 2;
     const int wide = FEW_WARPS / S * 16;
-    const int grid = (int)std::min<long long>(high * ((a.N + wide - 1) / wide), 8LL * ctx->sm_count);
-    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, 4 * ((size_t)a.experts + 1), 1, stream, a, S);
+    const long long items = high * ((a.N + wide - 1) / wide);
+    if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
+    const int grid = (int)std::min<long long>(items, 8LL * ctx->sm_count);
+    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, S);
 }
 
 int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale, int q_rows,
@@ -664,7 +724,6 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const long long rows = (long long)places / w->experts;
     if (q_rows == 0 || rows <= 8) return launch_few<1>(ctx, a, st);
     if (rows <= 16) return launch_few<2>(ctx, a, st);
-    if (rows <= 32) return launch_few<4>(ctx, a, st);
     const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
     if (tiles >= ctx->sm_count / 2) return launch_tc<256, 2>(ctx, a, st);
     if (tiles * 4 >= ctx->sm_count) return launch_tc<128, 1>(ctx, a, st);

@@ -16,7 +16,7 @@ struct RouteArgs {
     const float* bias;
     int32_t* experts;
     float* weights;
-    int T, E, top_k, sigmoid, groups, group_size, top_groups, group_top, renormalise, glog;
+    int T, E, top_k, sigmoid, groups, group_size, top_groups, group_top, renormalise, glog, per, vec;
     float scale;
 };
 
@@ -31,37 +31,74 @@ struct Choice {
     int mine;       // lane j: the expert of slot j, -1: none
     float top;      // softmax: the largest logit, and the sum of exp(logit - top)
     float sum;
-    bool certain;   // false: keys lie closer together than their rounding; nothing else is valid then
+    bool certain;   // false: only the 64-bit form over all experts can tell
 };
 
-// A group's experts lie on the 32 / 2^glog lanes of the group, up to NPL a lane: register r holds expert group * group_size +
-// r * L + (lane % L).  Without groups that is lane + 32 * r.
+// A group's experts lie on the 32 / 2^glog lanes of the group, `per` neighbours a lane (at most NPL, in registers 0 ..).
 struct Lanes {
-    int L, group, e0;  // lanes of a group, this lane's group, its first expert
-    __device__ __forceinline__ Lanes(const RouteArgs& p, int lane, int glog) : L(32 >> glog), group(lane >> (5 - glog)), e0(group * p.group_size + (lane & (L - 1))) {}
-    __device__ __forceinline__ bool there(const RouteArgs& p, int r) const { return group < p.groups && r * L + (e0 - group * p.group_size) < p.group_size; }
+    int L, group, e0, have;  // lanes of a group, this lane's group, its first expert, how many it has
+    __device__ __forceinline__ Lanes(const RouteArgs& p, int lane) : L(32 >> p.glog), group(lane >> (5 - p.glog)) {
+        const int in = (lane & (L - 1)) * p.per;
+        e0 = group * p.group_size + in;
+        have = group < p.groups ? min(max(p.group_size - in, 0), p.per) : 0;
+    }
 };
+// Values first .. first + NPL - 1 of a row, those past `have` as -inf.  vec: four at a time (rows and `have` allow it).
+template <typename T, int NPL>
+__device__ __forceinline__ void load_values(const T* at, int have, bool vec, float (&v)[NPL]) {
+    if (NPL >= 4 && vec) {
+#pragma unroll
+        for (int r = 0; r + 3 < NPL; r += 4) {
+            v[r] = v[r + 1] = v[r + 2] = v[r + 3] = -INFINITY;
+            if (r < have) {
+                if constexpr (sizeof(T) == 4) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(at + r));
+                    v[r] = f.x; v[r + 1] = f.y; v[r + 2] = f.z; v[r + 3] = f.w;
+                } else {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(at + r));
+                    const unsigned short h[4] = {(unsigned short)u.x, (unsigned short)(u.x >> 16), (unsigned short)u.y, (unsigned short)(u.y >> 16)};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[r + i] = to_f32(*reinterpret_cast<const T*>(&h[i]));
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < NPL; r++) v[r] = r < have ? to_f32(at[r]) : -INFINITY;
+    }
+}
 
-// A score in fp32 by the fast exponential and quotient, or in 64 bits.
-__device__ __forceinline__ float score_of(const RouteArgs& p, float l, float top, float all) {
-    return p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : __fdividef(__expf(l - top), all);
-}
-__device__ __forceinline__ double score_of(const RouteArgs& p, double l, double top, double all) {
-    return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / all;
-}
 __device__ __forceinline__ float warp_max(float v) {
     float r;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
+// (bits in an order that integers share: first the high words' largest, then the low words' among its lanes)
 __device__ __forceinline__ double warp_max(double v) {
-    for (int d = 16; d; d >>= 1) v = fmax(v, __shfl_xor_sync(FULL, v, d));
-    return v;
+    long long b = __double_as_longlong(v + 0.0);  // -0 as +0
+    b ^= (b >> 63) & 0x7FFFFFFFFFFFFFFFLL;
+    const int hi = (int)(b >> 32), top = __reduce_max_sync(FULL, hi);
+    const unsigned low = __reduce_max_sync(FULL, hi == top ? (unsigned)b : 0u);
+    b = (long long)top << 32 | low;
+    b ^= (b >> 63) & 0x7FFFFFFFFFFFFFFFLL;
+    return __longlong_as_double(b);
+}
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// A score in fp32 by the fast exponential and quotient, or in 64 bits.
+__device__ __forceinline__ float score_of(const RouteArgs& p, float l, float top, float all) {
+    return p.sigmoid ? reciprocal(1.0f + __expf(-l)) : __expf(l - top) * reciprocal(all);
+}
+__device__ __forceinline__ double score_of(const RouteArgs& p, double l, double top, double all) {
+    return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / all;
 }
 // The two best values of a group, (a, b) being those of its lanes, and whether the group is among the best: groups ranked by a, or by
 // a + b.  Returns the group's worth.
 template <typename Key>
-__device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, int glog, Key a, Key b, bool& kept) {
+__device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, Key a, Key b, bool& kept) {
     for (int d = 1; d < at.L; d <<= 1) {
         const Key oa = __shfl_xor_sync(FULL, a, d), ob = __shfl_xor_sync(FULL, b, d);
         b = fmax(fmin(a, oa), fmax(b, ob));
@@ -70,7 +107,7 @@ __device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, i
     const Key none = -INFINITY, worth = p.group_top == 2 && b != none ? a + b : a;
     int better = 0;
     for (int g = 0; g < p.groups; g++) {
-        const Key o = __shfl_sync(FULL, worth, g << (5 - glog));
+        const Key o = __shfl_sync(FULL, worth, g << (5 - p.glog));
         better += o > worth || (o == worth && g < at.group);
     }
     kept = at.group < p.groups && better < p.top_groups;
@@ -79,14 +116,14 @@ __device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, i
 
 // The choice in 64 bits.
 template <typename T, int NPL>
-__device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int lane, int glog) {
-    const Lanes at(p, lane, glog);
+__device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int lane) {
+    const Lanes at(p, lane);
     const double none = -INFINITY;
     double key[NPL];
     double top = none;
 #pragma unroll
     for (int r = 0; r < NPL; r++) {
-        const float l = at.there(p, r) ? to_f32(row[at.e0 + r * at.L]) : -INFINITY;
+        const float l = r < at.have ? to_f32(row[at.e0 + r]) : -INFINITY;
         key[r] = barred(l) ? none : (double)bounded(l);
         top = fmax(top, key[r]);
     }
@@ -94,11 +131,11 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
     double all = 0;
     if (!p.sigmoid && top > none) {
 #pragma unroll 1
-        for (int r = 0; r < NPL; r++)  // (from memory again: a register array cannot be indexed)
-            if (at.there(p, r)) {
-                const float l = to_f32(row[at.e0 + r * at.L]);
-                if (!barred(l)) all += exp((double)bounded(l) - top);
-            }
+        for (int r = 0; r < at.have; r++) {  // (from memory again: a register array cannot be indexed)
+            const float l = to_f32(row[at.e0 + r]);
+            if (!barred(l)) all += exp((double)bounded(l) - top);
+        }
+        __syncwarp();
         for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(FULL, all, d);
     }
     const bool grouped = p.top_groups < p.groups;
@@ -109,7 +146,7 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
         if (v != none && (p.bias || (grouped && p.group_top == 2))) {
             v = score_of(p, v, top, all);
             if (p.bias) {
-                const float c = __ldg(p.bias + at.e0 + r * at.L);
+                const float c = __ldg(p.bias + at.e0 + r);
                 key[r] = v = barred(c) ? none : v + (double)bounded(c);
             }
         }
@@ -118,7 +155,7 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
     }
     if (grouped) {
         bool kept;
-        rank_group<double>(p, at, glog, a, b, kept);
+        rank_group<double>(p, at, a, b, kept);
         if (!kept) {
 #pragma unroll
             for (int r = 0; r < NPL; r++) key[r] = none;
@@ -130,57 +167,89 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
         int e = MAX_E;
 #pragma unroll
         for (int r = 0; r < NPL; r++)
-            if (key[r] > best) { best = key[r]; e = at.e0 + r * at.L; }
+            if (key[r] > best) { best = key[r]; e = at.e0 + r; }
         const double m = warp_max(best);
         if (m == none) break;
         e = (int)__reduce_min_sync(FULL, best == m ? (unsigned)e : (unsigned)MAX_E);
         if (lane == j) mine = e;
 #pragma unroll
         for (int r = 0; r < NPL; r++)
-            if (at.e0 + r * at.L == e) key[r] = none;
+            if (at.e0 + r == e) key[r] = none;
     }
     return mine;
+}
+
+// The candidates' order in 64 bits: lane j < n has expert `mine` (MAX_E: none) of logit l and bias b.  Returns the expert of place j.
+template <typename T>
+__device__ __noinline__ int order_exact(const RouteArgs& p, const T* row, int lane, int n, int mine, float l, float b, float top) {
+    double key = (double)bounded(l);
+    if (p.bias) {
+        double all = 1;
+        if (!p.sigmoid) {
+            all = 0;
+            for (int e = lane; e < p.E; e += 32) {
+                const float v = to_f32(row[e]);
+                if (!barred(v)) all += exp((double)bounded(v) - (double)top);
+            }
+            for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(FULL, all, d);
+        }
+        key = score_of(p, key, (double)top, all) + (double)bounded(b);
+    }
+    int place = 0, result = MAX_E;
+    for (int i = 0; i < n; i++) {
+        const double o = __shfl_sync(FULL, key, i);
+        const int e = __shfl_sync(FULL, mine, i);
+        place += e < MAX_E && (o > key || (o == key && e < mine));
+    }
+    for (int i = 0; i < n; i++) {
+        const int at = __shfl_sync(FULL, place, i), e = __shfl_sync(FULL, mine, i);
+        if (at == lane && e < MAX_E) result = e;
+    }
+    return result;
 }
 
 // The choice for one token by one warp, in fp32.  Every lane sorts its keys, and the warp takes the best of the lanes' first ones,
 // top_k times.  A key carries its register's number in its lowest bits (LOG of them), lower registers above higher ones.
 //
-// The choice is certain unless two keys that have to be told apart are closer than their errors; the token is then chosen in 64
-// bits.  A score by the fast functions is off by 2^-22 from the exponential and by the rounding of its argument, of which a score (at
+// That is certain unless two keys that have to be told apart are closer than their errors.  Experts that are near each other are then
+// ordered in 64 bits, and a token whose groups are is chosen in 64 bits altogether.  A score by the fast functions is off by 2^-22 from the exponential and by the rounding of its argument, of which a score (at
 // most 1, and s * d <= 1 / e) keeps 2^-22 together; a softmax's sum adds NPL + 5 roundings of 2^-24, the quotient 2^-22, the bias
 // |key| * 2^-24.  A key without a bias is the logit itself.  The register's number takes LOG bits.  Two keys are in order if they
 // differ by (NPL + 24) * 2^-23 + |key| * 2^(LOG - 21) (first term: with a bias), or if they are made of the same logit and the same
 // bias and come in their experts' order.
 template <typename T, int NPL>
-__device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int lane, int glog) {
+__device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int lane) {
     constexpr int LOG = NPL == 2 ? 1 : NPL == 4 ? 2 : NPL == 8 ? 3 : NPL == 16 ? 4 : NPL == 32 ? 5 : 6;
-    const Lanes at(p, lane, glog);
+    const Lanes at(p, lane);
     Choice c;
     float key[NPL];
+    load_values<T, NPL>(row + at.e0, at.have, p.vec, key);
     float top = -INFINITY;
 #pragma unroll
     for (int r = 0; r < NPL; r++) {
-        float l = -INFINITY;
-        if (at.there(p, r)) l = to_f32(row[at.e0 + r * at.L]);
-        key[r] = barred(l) ? -INFINITY : bounded(l);
+        key[r] = barred(key[r]) ? -INFINITY : bounded(key[r]);
         top = fmaxf(top, key[r]);
     }
-    c.top = warp_max(top);
-    c.sum = 0.f;
-    if (!p.sigmoid && c.top > -INFINITY) {
-        float sum = 0.f;
+    c.top = c.sum = 0.f;
+    if (!p.sigmoid) {
+        c.top = warp_max(top);
+        if (c.top > -INFINITY) {
+            float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < NPL; r++) sum += __expf(key[r] - c.top);  // exp(-inf) = 0
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(FULL, sum, d);
-        c.sum = sum;
+            for (int r = 0; r < NPL; r++) sum += __expf(key[r] - c.top);  // exp(-inf) = 0
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(FULL, sum, d);
+            c.sum = sum;
+        }
     }
     if (p.bias) {
+        float b[NPL];
+        load_values<float, NPL>(p.bias + at.e0, at.have, p.vec, b);
+        const float inverse = reciprocal(c.sum);
 #pragma unroll
-        for (int r = 0; r < NPL; r++)
-            if (key[r] != -INFINITY) {
-                const float b = __ldg(p.bias + at.e0 + r * at.L);
-                key[r] = barred(b) ? -INFINITY : score_of(p, key[r], c.top, c.sum) + bounded(b);
-            }
+        for (int r = 0; r < NPL; r++) {
+            const float s = p.sigmoid ? reciprocal(1.0f + __expf(-key[r])) : __expf(key[r] - c.top) * inverse;
+            key[r] = key[r] == -INFINITY || barred(b[r]) ? -INFINITY : s + bounded(b[r]);
+        }
     }
     // the register's number: a larger one makes a key smaller, whatever its sign; infinity keeps its bits
 #pragma unroll
@@ -210,48 +279,61 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
         float a = key[0], b = key[1];
         const bool sums = p.group_top == 2 && !p.bias;
         if (sums) {  // experts are ranked by their logits, groups by scores
-            if (a != -INFINITY) a = score_of(p, bounded(to_f32(row[at.e0 + register_of(a) * at.L])), c.top, c.sum);
-            if (b != -INFINITY) b = score_of(p, bounded(to_f32(row[at.e0 + register_of(b) * at.L])), c.top, c.sum);
+            if (a != -INFINITY) a = score_of(p, bounded(to_f32(row[at.e0 + register_of(a)])), c.top, c.sum);
+            if (b != -INFINITY) b = score_of(p, bounded(to_f32(row[at.e0 + register_of(b)])), c.top, c.sum);
         }
         bool kept;
-        const float worth = rank_group<float>(p, at, glog, a, b, kept);
+        const float worth = rank_group<float>(p, at, a, b, kept);
         // the worst group that is kept against the best that is not
         const float best_out = warp_max(kept || at.group >= p.groups ? -INFINITY : worth), worst_in = -warp_max(kept ? -worth : -INFINITY);
         // (a score made of a logit that lost LOG bits is off by |logit| times that; s * |logit| <= s * |top| + 1 / e)
         const float lost = sums ? (1.0f + (p.sigmoid ? 0.f : fabsf(c.top) * fabsf(worst_in))) * tol1 : 0.f;
-        const float tol = 4 * ((NPL + 24) * 0x1p-23f * (p.bias || sums) + fmaxf(fabsf(worst_in), fabsf(best_out)) * tol1 + lost) + 1e-30f;
+        const float tol = 2 * ((NPL + 24) * 0x1p-23f * (p.bias || sums) + fmaxf(fabsf(worst_in), fabsf(best_out)) * (tol1 + 0x1p-22f) + lost) + 1e-30f;  // (a worth is made of two)
         certain = best_out == -INFINITY || worst_in - best_out > tol;
         if (!kept) key[0] = -INFINITY;
     }
-    c.mine = -1;
-    float last = 0.f;
-    int last_e = -1;
-    for (int j = 0; j < MAX_E; j++) {
+    // lane j < n: the j-th best key and its expert
+    float mine_key = -INFINITY;
+    int mine = MAX_E, n = p.top_k, first = at.e0 + register_of(key[0]);
+    auto pop = [&](int j) {
         const float m = warp_max(key[0]);
-        const bool close = j > 0 && near(last, m);
-        if (m == -INFINITY || (j >= p.top_k && !close)) break;
-        const int mine = at.e0 + register_of(key[0]) * at.L;
-        const int e = (int)__reduce_min_sync(FULL, key[0] == m ? (unsigned)mine : (unsigned)MAX_E);
-        if (e >= p.E) {
-            certain = false;
-            break;
+        const int e = (int)__reduce_min_sync(FULL, key[0] == m ? (unsigned)first : (unsigned)MAX_E);
+        if (lane == j) {
+            mine_key = m;
+            mine = e;
         }
-        if (close) {
-            const bool same = e > last_e && to_f32(row[e]) == to_f32(row[last_e]) && (!p.bias || __ldg(p.bias + e) == __ldg(p.bias + last_e));
-            if (!same) {
-                certain = false;
-                break;
-            }
-        }
-        if (lane == j && j < p.top_k) c.mine = e;
-        last = m;
-        last_e = e;
-        if (key[0] == m && mine == e) {
+        if (key[0] == m && first == e) {
 #pragma unroll
             for (int r = 0; r + 1 < NPL; r++) key[r] = key[r + 1];
             key[NPL - 1] = -INFINITY;
+            first = at.e0 + register_of(key[0]);
         }
+    };
+    for (int j = 0; j < n; j++) pop(j);
+    // those behind the last slot that are near it, and near each other, are candidates too
+    float last = __shfl_sync(FULL, mine_key, n - 1);
+    for (;;) {
+        const float m = warp_max(key[0]);
+        if (m == -INFINITY || !near(last, m)) break;
+        if (n == 32) {
+            certain = false;
+            break;
+        }
+        pop(n++);
+        last = m;
     }
+    // in order?  Where two neighbours are near each other, they have to be the same and to come in their experts' order.
+    float l = 0.f, b = 0.f;
+    if (mine_key != -INFINITY && mine < p.E) {
+        l = to_f32(row[mine]);
+        if (p.bias) b = __ldg(p.bias + mine);
+    }
+    const float prev_key = __shfl_up_sync(FULL, mine_key, 1), prev_l = __shfl_up_sync(FULL, l, 1), prev_b = __shfl_up_sync(FULL, b, 1);
+    const int prev = __shfl_up_sync(FULL, mine, 1);
+    if (__any_sync(FULL, mine_key != -INFINITY && mine >= p.E)) certain = false;
+    const bool odd = lane > 0 && lane < n && mine_key != -INFINITY && near(prev_key, mine_key) && !(mine > prev && l == prev_l && b == prev_b);
+    if (__any_sync(FULL, odd) && certain) mine = order_exact<T>(p, row, lane, n, mine_key != -INFINITY ? mine : MAX_E, l, b, c.top);
+    c.mine = mine_key != -INFINITY && lane < p.top_k && mine < p.E ? mine : -1;
     c.certain = certain;
     return c;
 }
@@ -282,41 +364,6 @@ struct PlanArgs {
     int32_t* rows;
     int32_t* slots;
 };
-// Pairs are cut into one run for each warp.
-__device__ __forceinline__ int2 run_of(int pairs, int warp, int warps) {
-    const long long each = (((long long)pairs + warps - 1) / warps + 31) & ~31LL;
-    const long long a = min(warp * each, (long long)pairs);
-    return make_int2((int)a, (int)min(a + each, (long long)pairs));
-}
-// s_hist[w][e] = pairs of expert e in the run of the block's warp w.  Ends with a barrier.
-__device__ __forceinline__ void count_runs(const int32_t* experts, int2 run, int E, int* s_hist, int tid, int threads) {
-    const int warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
-    for (int i = tid; i < warps * E; i += threads) s_hist[i] = 0;
-    __syncthreads();
-    for (int i = run.x + lane; i < run.y; i += 32) {
-        const int e = experts[i];
-        if (e >= 0) atomicAdd(&s_hist[warp * E + e], 1);  // (whole numbers: the order of the additions does not matter)
-    }
-    __syncthreads();
-}
-// Places of a warp's pairs, s_hist[w][e] = the first place of warp w's pairs of expert e.
-__device__ __forceinline__ void place_runs(const int32_t* experts, int2 run, int top_k, int E, int* s_hist, const PlanArgs& o, int tid) {
-    const int warp = tid >> 5, lane = tid & 31;
-    for (int base = run.x; base < run.y; base += 32) {
-        const int i = base + lane;
-        const int e = i < run.y ? experts[i] : -1;
-        const unsigned alike = __match_any_sync(FULL, e);
-        int at = -1;
-        if (e >= 0) at = s_hist[warp * E + e] + __popc(alike & ((1u << lane) - 1));
-        __syncwarp();
-        if (e >= 0 && (alike >> lane) == 1u) s_hist[warp * E + e] = at + 1;  // the last of the alike
-        __syncwarp();
-        if (i < run.y) {
-            o.slots[i] = at;
-            if (e >= 0) o.rows[at] = i / top_k;
-        }
-    }
-}
 // Exclusive sums of s_v[0 .. n) by the whole block; s_v[n] = the total.
 __device__ __forceinline__ void scan_block(int* s_v, int n, int* s_part, int tid, int threads) {
     const int lane = tid & 31, warp = tid >> 5;
@@ -342,80 +389,131 @@ __device__ __forceinline__ void scan_block(int* s_v, int n, int* s_part, int tid
     __syncthreads();
 }
 
-// The order of the pairs by a cluster of RANKS blocks (1: no cluster): every warp counts its run, every block adds up its warps' and
-// reads the other blocks' counts from their shared memory, and every warp places its run.  s_hist: [warps][E], [E] counts of the
-// block, [E + 1] first places.
+// The order of the pairs by a cluster of RANKS blocks (1: no cluster), each with an equal part of the tokens.  A token takes an expert
+// at most once, so 32 neighbouring tokens' pairs with an expert are the bits of one word; a pair's place among its expert's is the
+// number of bits before its own.  Each block goes over its tokens in slabs of `high` groups of 32; where one slab does not hold them
+// all, once to count and once more to place.  Shared memory: masks [high][E], bits before them [high][E], [E] counts of the block,
+// [E + 1] first places, [E] pairs of the blocks before.
+constexpr size_t plan_smem(int high, int E) { return sizeof(int) * ((size_t)(2 * high + 3) * E + 1); }
 template <int RANKS, int THREADS>
-__device__ __forceinline__ void plan_pairs(const int32_t* experts, int pairs, int top_k, int E, const PlanArgs& o, int* s_hist, int* s_part, int tid) {
-    constexpr int WARPS = THREADS / 32;
-    int *s_count = s_hist + WARPS * E, *s_first = s_count + E;
+__device__ __forceinline__ void plan_pairs(const RouteArgs& p, const PlanArgs& o, int high, int* smem, int* s_part, int tid) {
+    const int E = p.E, k = p.top_k;
+    unsigned* s_mask = reinterpret_cast<unsigned*>(smem);
+    int *s_before = smem + high * E, *s_count = s_before + high * E, *s_first = s_count + E, *s_below = s_first + E + 1;
     const int rank = RANKS > 1 ? (int)cluster_ctarank() : 0;
-    const int2 run = run_of(pairs, rank * WARPS + (tid >> 5), RANKS * WARPS);
-    count_runs(experts, run, E, s_hist, tid, THREADS);
-    for (int e = tid; e < E; e += THREADS) {
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            const int v = s_hist[w * E + e];
-            s_hist[w * E + e] = sum;
-            sum += v;
-        }
-        s_count[e] = sum;
-    }
-    if (RANKS > 1) cluster_sync_all(); else __syncthreads();
-    for (int e = tid; e < E; e += THREADS) {
-        int all = 0, below = 0;
-#pragma unroll
-        for (int r = 0; r < RANKS; r++) {
-            int v;
-            if (RANKS > 1) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(s_count + e), r)) : "memory");
-            else v = s_count[e];
-            all += v;
-            if (r < rank) below += v;
-        }
-        s_first[e] = all;
-        for (int w = 0; w < WARPS; w++) s_hist[w * E + e] += below;
-    }
+    const long long groups = ((long long)p.T + 31) / 32, each = (groups + RANKS - 1) / RANKS;
+    const long long g0 = min(rank * each, groups), g1 = min(g0 + each, groups);
+    const bool once = g1 - g0 <= high;
+    for (int e = tid; e < E; e += THREADS) s_count[e] = s_below[e] = 0;
     __syncthreads();
-    scan_block(s_first, E, s_part, tid, THREADS);
-    for (int i = tid; i < WARPS * E; i += THREADS) s_hist[i] += s_first[i % E];
-    if (rank == 0)
-        for (int e = tid; e <= E; e += THREADS) o.offsets[e] = s_first[e];
-    __syncthreads();
-    place_runs(experts, run, top_k, E, s_hist, o, tid);
-    for (int i = s_first[E] + rank * THREADS + tid; i < pairs && i >= 0; i += RANKS * THREADS) o.rows[i] = -1;
+    auto place_of = [&](int i, int t0, int e) {  // pair i of expert e, of the slab that begins with token t0
+        const int t = (int)((unsigned)i / (unsigned)k) - t0;
+        return s_before[(t >> 5) * E + e] + __popc(s_mask[(t >> 5) * E + e] & ((1u << (t & 31)) - 1));
+    };
+    for (int pass = 0; pass < 2; pass++) {
+        for (long long g = g0; g < g1; g += high) {
+            const int here = (int)min((long long)high, g1 - g), t0 = (int)(g * 32), i0 = t0 * k, i1 = (int)min((long long)t0 + here * 32, (long long)p.T) * k;
+            if (pass == 0 || !once) {
+                for (int i = tid; i < here * E; i += THREADS) s_mask[i] = 0;
+                __syncthreads();
+                for (int i = i0 + tid; i < i1; i += 4 * THREADS) {
+                    int e[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) e[u] = i + u * THREADS < i1 ? p.experts[i + u * THREADS] : -1;
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        if (e[u] >= 0) {
+                            const int t = (int)((unsigned)(i + u * THREADS) / (unsigned)k) - t0;
+                            atomicOr(&s_mask[(t >> 5) * E + e[u]], 1u << (t & 31));
+                        }
+                }
+                __syncthreads();
+                for (int e = tid; e < E; e += THREADS) {
+                    int sum = pass == 0 ? s_count[e] : s_below[e];
+#pragma unroll 8
+                    for (int h = 0; h < here; h++) {
+                        s_before[h * E + e] = sum;
+                        sum += __popc(s_mask[h * E + e]);
+                    }
+                    (pass == 0 ? s_count : s_below)[e] = sum;
+                }
+                __syncthreads();
+            }
+            if (pass == 1)
+                for (int i = i0 + tid; i < i1; i += 4 * THREADS) {
+                    int e[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) e[u] = i + u * THREADS < i1 ? p.experts[i + u * THREADS] : -1;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int j = i + u * THREADS;
+                        if (j >= i1) break;
+                        int at = -1;
+                        if (e[u] >= 0) {
+                            at = s_first[e[u]] + (once ? s_below[e[u]] : 0) + place_of(j, t0, e[u]);
+                            o.rows[at] = (int)((unsigned)j / (unsigned)k);
+                        }
+                        o.slots[j] = at;
+                    }
+                }
+            __syncthreads();
+        }
+        if (pass == 1) break;
+        if (RANKS > 1) {
+            cluster_sync_all();
+            for (int e = tid; e < E; e += THREADS) {
+                int v[RANKS], all = 0, below = 0;
+#pragma unroll
+                for (int r = 0; r < RANKS; r++) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[r]) : "r"(mapa_shared(smem_u32(s_count + e), r)) : "memory");
+#pragma unroll
+                for (int r = 0; r < RANKS; r++) {
+                    all += v[r];
+                    if (r < rank) below += v[r];
+                }
+                s_first[e] = all;
+                s_below[e] = below;
+            }
+        } else {
+            for (int e = tid; e < E; e += THREADS) s_first[e] = s_count[e];
+        }
+        __syncthreads();
+        scan_block(s_first, E, s_part, tid, THREADS);
+        if (rank == 0)
+            for (int e = tid; e <= E; e += THREADS) o.offsets[e] = s_first[e];
+    }
+    const int pairs = p.T * k;
+    for (long long i = (long long)s_first[E] + rank * THREADS + tid; i < pairs; i += RANKS * THREADS) o.rows[i] = -1;
     if (RANKS > 1) cluster_sync_all();  // no block leaves while another may read its counts
 }
 
 constexpr int ROUTE_WARPS = 16, PLAN_RANKS = 8, PLAN_THREADS = 1024;
-constexpr size_t plan_smem(int warps, int E) { return sizeof(int) * ((size_t)(warps + 2) * E + 1); }
 
 // One warp a token.  PLAN: one block takes all tokens and orders the pairs as well.
 template <typename T, int NPL, bool PLAN>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32, NPL <= 16 ? 2 : 1) route_kernel(RouteArgs p, PlanArgs o) {
-    extern __shared__ int s_hist[];
+__global__ void __launch_bounds__(ROUTE_WARPS * 32, NPL <= 16 ? 2 : 1) route_kernel(const __grid_constant__ RouteArgs p, const __grid_constant__ PlanArgs o) {
+    extern __shared__ int s_plan[];
     __shared__ int s_part[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (long long t = (long long)blockIdx.x * ROUTE_WARPS + warp; t < p.T; t += (long long)gridDim.x * ROUTE_WARPS) {
         const T* row = (const T*)p.logits + t * p.stride;
-        Choice c = choose<T, NPL>(p, row, lane, p.glog);
-        if (!c.certain) c.mine = choose_exact<T, NPL>(p, row, lane, p.glog);
+        Choice c = choose<T, NPL>(p, row, lane);
+        if (!c.certain) c.mine = choose_exact<T, NPL>(p, row, lane);
         finish_token(p, row, t, lane, c);
     }
     if (PLAN) {
         __syncthreads();
-        plan_pairs<1, ROUTE_WARPS * 32>(p.experts, p.T * p.top_k, p.top_k, p.E, o, s_hist, s_part, tid);
+        plan_pairs<1, ROUTE_WARPS * 32>(p, o, 1, s_plan, s_part, tid);
     }
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(RouteArgs p, PlanArgs o) {
-    extern __shared__ int s_hist[];
+__global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const __grid_constant__ RouteArgs p, const __grid_constant__ PlanArgs o, int high) {
+    extern __shared__ int s_plan[];
     __shared__ int s_part[32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    plan_pairs<PLAN_RANKS, PLAN_THREADS>(p.experts, p.T * p.top_k, p.top_k, p.E, o, s_hist, s_part, threadIdx.x);
+    plan_pairs<PLAN_RANKS, PLAN_THREADS>(p, o, high, s_plan, s_part, threadIdx.x);
 }
 
 template <typename... Args>
@@ -446,6 +544,7 @@ int launch(void (*kern)(Args...), int grid, int threads, size_t smem, int cluste
 // Tokens that one block chooses and orders in one launch (two for each of its warps); more are chosen by many blocks and ordered by
 // a second launch.
 constexpr int ONE_BLOCK_TOKENS = 2 * ROUTE_WARPS;
+static_assert(ONE_BLOCK_TOKENS <= 32, "one group of tokens");
 
 // Dynamic shared memory past 48 KB, once per kernel and device.
 template <typename... Args>
@@ -460,21 +559,21 @@ int allow_smem(void (*kern)(Args...), size_t bytes, bool (&set)[64], int device)
 template <typename T, int NPL>
 int launch_route(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, bool plan, cudaStream_t st) {
     int rc;
-    if (plan && a.T <= ONE_BLOCK_TOKENS) {
-        static bool set[64] = {false};
-        if ((rc = allow_smem(route_kernel<T, NPL, true>, plan_smem(ROUTE_WARPS, MAX_E), set, ctx->device))) return rc;
-        return launch<RouteArgs, PlanArgs>(route_kernel<T, NPL, true>, 1, ROUTE_WARPS * 32, plan_smem(ROUTE_WARPS, a.E), 1, st, a, o);
-    }
+    if (plan && a.T <= ONE_BLOCK_TOKENS) return launch<RouteArgs, PlanArgs>(route_kernel<T, NPL, true>, 1, ROUTE_WARPS * 32, plan_smem(1, a.E), 1, st, a, o);
     const int blocks = std::min((a.T + ROUTE_WARPS - 1) / ROUTE_WARPS, (NPL <= 16 ? 2 : 1) * ctx->sm_count);
     if ((rc = launch<RouteArgs, PlanArgs>(route_kernel<T, NPL, false>, blocks, ROUTE_WARPS * 32, 0, 1, st, a, o)) || !plan) return rc;
     static bool set[64] = {false};
-    if ((rc = allow_smem(plan_kernel, plan_smem(PLAN_THREADS / 32, MAX_E), set, ctx->device))) return rc;
-    return launch<RouteArgs, PlanArgs>(plan_kernel, PLAN_RANKS, PLAN_THREADS, plan_smem(PLAN_THREADS / 32, a.E), PLAN_RANKS, st, a, o);
+    constexpr size_t MOST = 200 * 1024;
+    if ((rc = allow_smem(plan_kernel, MOST, set, ctx->device))) return rc;
+    // groups of 32 tokens that a block holds at a time: all of its own, or as many as fit
+    const int own = (int)((((long long)a.T + 31) / 32 + PLAN_RANKS - 1) / PLAN_RANKS), fit = (int)((MOST / sizeof(int) / a.E - 4) / 2);
+    const int high = std::min(own, fit);
+    return launch<RouteArgs, PlanArgs, int>(plan_kernel, PLAN_RANKS, PLAN_THREADS, plan_smem(high, a.E), PLAN_RANKS, st, a, o, high);
 }
 // Registers a lane needs for its share of the experts.
 template <typename T>
 int launch_route_npl(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, bool plan, cudaStream_t st) {
-    const int lanes = 32 >> a.glog, npl = (a.group_size + lanes - 1) / lanes;
+    const int npl = a.per;
     if (npl <= 2) return launch_route<T, 2>(ctx, a, o, plan, st);
     if (npl <= 4) return launch_route<T, 4>(ctx, a, o, plan, st);
     if (npl <= 8) return launch_route<T, 8>(ctx, a, o, plan, st);
@@ -505,7 +604,7 @@ int tnns_cuda_route(tnns_cuda_ctx* ctx, const tnns_route_t* r, const void* d_log
     int rc = check_route(r);
     if (rc) return rc;
     if (!tnns_dtype_ok(dtype)) return tnns_fail(TNNS_ERR_INVALID, "unknown element type %d", dtype);
-    if (T < 0 || (long long)T * r->top_k > 0x7FFFFFFFLL) return tnns_fail(TNNS_ERR_INVALID, "bad size: %d tokens, top_k %d", T, r->top_k);
+    if (T < 0 || (long long)T * r->top_k > 0x7FFF0000LL) return tnns_fail(TNNS_ERR_INVALID, "bad size: %d tokens, top_k %d", T, r->top_k);
     if (stride < r->experts) return tnns_fail(TNNS_ERR_INVALID, "rows of %d logits at a stride of %lld", r->experts, stride);
     const bool plan = d_offsets || d_rows || d_slots;
     if (plan && !d_offsets) return tnns_fail(TNNS_ERR_INVALID, "the order of the pairs needs offsets, rows and slots");
@@ -522,6 +621,11 @@ int tnns_cuda_route(tnns_cuda_ctx* ctx, const tnns_route_t* r, const void* d_log
     a.top_groups = r->top_groups < r->groups ? r->top_groups : 1;
     a.group_size = r->experts / a.groups; a.group_top = r->group_top;
     for (a.glog = 0; (1 << a.glog) < a.groups;) a.glog++;
+    // experts of a lane; four at a time where rows, groups and lanes all begin on a multiple of four
+    const int lanes = 32 >> a.glog, eb = tnns_dtype_bytes(dtype);
+    a.per = (a.group_size + lanes - 1) / lanes;
+    a.vec = a.per > 2 && a.group_size % 4 == 0 && stride % 4 == 0 && (uintptr_t)d_logits % (4 * eb) == 0 && (uintptr_t)d_bias % 16 == 0;
+    if (a.vec) a.per = (a.per + 3) / 4 * 4;
     a.renormalise = r->renormalise; a.scale = r->scale;
     const cudaStream_t st = (cudaStream_t)stream;
     if (T == 0) {

@@ -4,6 +4,7 @@
 
 #include "dtype.cuh"
 #include "internal.h"
+#include "mbar.cuh"
 
 namespace {
 
@@ -36,6 +37,17 @@ __device__ __forceinline__ void unpack(const Chunk<__nv_bfloat16>& c, float (&f)
         f[2 * j + 1] = __uint_as_float(c.w[j] & 0xFFFF0000u);
     }
 }
+// The 16 bytes from byte `off` on of the 32 that a and b hold.
+template <typename T>
+__device__ __forceinline__ void realign(const uint4& a, const uint4& b, int off, uint32_t (&w)[4]) {
+    uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 7; j++) v[j] = off & 4 ? v[j + 1] : v[j];
+#pragma unroll
+    for (int j = 0; j < 5; j++) v[j] = off & 8 ? v[j + 2] : v[j];
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = sizeof(T) == 4 ? v[j] : __funnelshift_r(v[j], v[j + 1], (off & 2) * 8);
+}
 // Chunk i of a row of K elements, zeros past the row's end.  MIS: rows need not start on 16 bytes; the two aligned vectors that
 // overlap the chunk are fetched (the second only where it holds elements of the row, so that no other 16 bytes than those that
 // the row touches are read) and shifted together.
@@ -52,16 +64,7 @@ __device__ __forceinline__ Chunk<T> load_chunk(const T* row, int i, int K) {
         const uint4 a = base[0];
         uint4 b = make_uint4(0, 0, 0, 0);
         if (off && ((long long)(i + 1) * 16 - off) < (long long)K * (int)sizeof(T)) b = base[1];
-        const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        uint32_t u[5];
-        switch (off >> 2) {
-            case 0: u[0] = v[0]; u[1] = v[1]; u[2] = v[2]; u[3] = v[3]; u[4] = v[4]; break;
-            case 1: u[0] = v[1]; u[1] = v[2]; u[2] = v[3]; u[3] = v[4]; u[4] = v[5]; break;
-            case 2: u[0] = v[2]; u[1] = v[3]; u[2] = v[4]; u[3] = v[5]; u[4] = v[6]; break;
-            default: u[0] = v[3]; u[1] = v[4]; u[2] = v[5]; u[3] = v[6]; u[4] = v[7]; break;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) c.w[j] = sizeof(T) == 4 ? u[j] : __funnelshift_r(u[j], u[j + 1], (off & 2) * 8);
+        realign<T>(a, b, off, c.w);
     }
     const int have = K - i * VE;
     if (have < VE) {
@@ -166,9 +169,21 @@ __device__ __forceinline__ void store_chunk(int8_t* out, int i, int K, const uin
     }
 }
 
+template <typename T>
+__device__ __forceinline__ void finish_chunk(const Chunk<T>& c, int8_t* out, int i, int K, const RowScale& s) {
+    constexpr int VE = Chunk<T>::VE;
+    float f[VE];
+    uint32_t w[VE / 4];
+    unpack(c, f);
+    quantise_chunk<T, VE>(f, s, w);
+    store_chunk<VE>(out, i, K, w);
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // GROUP threads a row (a warp, or the whole block), which keeps the row in registers between its largest magnitude and its
-// integers, NV chunks a thread: every element is read once.  LONG: rows that do not fit; the chunks past the kept ones are
-// read a second time.  Bounded by memory: M = 8192, K = 4096 (figures beside the launch).
+// integers, NV chunks a thread: every element is read once.  LONG: rows that do not fit; the chunks past the kept ones are read a
+// second time.  The form for few rows (all latency) and for rows too long for the ring below.  (Groups that went on to another row and
+// requested it ahead were slower, 51 against 33 us for 8192 x 4096 bf16: their registers cost more rows in flight than that gave.)
 template <typename T, int GROUP, int NV, bool MIS, bool LONG>
 __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(const T* __restrict__ x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
                                                                               float* __restrict__ scale, int M, int K) {
@@ -176,10 +191,10 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
     __shared__ uint32_t s_top[32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int m = blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / GROUP : 0), lane = threadIdx.x % GROUP;
-    if (m >= M) return;  // (a whole group, and with ROWS > 1 a whole warp)
-    const T* row = x + (long long)m * x_stride;
-    const int chunks = (K + VE - 1) / VE;
+    const long long m = (long long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / GROUP : 0);
+    const int lane = threadIdx.x % GROUP, chunks = (K + VE - 1) / VE;
+    if (m >= M) return;  // (a whole group, and with several a whole warp)
+    const T* row = x + m * x_stride;
     Chunk<T> c[NV];
     uint32_t top = 0;
 #pragma unroll
@@ -197,27 +212,81 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
         bits = __reduce_max_sync(0xFFFFFFFFu, (threadIdx.x & 31) < GROUP / 32 ? s_top[threadIdx.x & 31] : 0u);
     }
     const RowScale s = row_scale(bits, lane == 0 ? scale + m : nullptr);
-    int8_t* out = q + (long long)m * q_stride;
-    auto finish = [&](const Chunk<T>& ch, int i) {
-        float f[VE];
-        uint32_t w[VE / 4];
-        unpack(ch, f);
-        quantise_chunk<T, VE>(f, s, w);
-        store_chunk<VE>(out, i, K, w);
-    };
+    int8_t* out = q + m * q_stride;
 #pragma unroll
     for (int v = 0; v < NV; v++)
-        if (lane + v * GROUP < chunks) finish(c[v], lane + v * GROUP);
+        if (lane + v * GROUP < chunks) finish_chunk(c[v], out, lane + v * GROUP, K, s);
     if (LONG)
-        for (int i = lane + NV * GROUP; i < chunks; i += GROUP) finish(load_chunk<T, MIS>(row, i, K), i);
+        for (int i = lane + NV * GROUP; i < chunks; i += GROUP) finish_chunk(load_chunk<T, MIS>(row, i, K), out, i, K, s);
+}
+
+// Many rows: persistent blocks, RING_WARPS warps, each with rows of its own that the copy engine brings into its slots of shared
+// memory (the aligned 16 bytes that the row touches), `slots` a warp, ahead of the warp's work: the bytes on their way do not
+// depend on registers.  A warp goes over its row twice, for the largest magnitude and for the integers.
+constexpr int RING_WARPS = 12, RING_MAX_SLOTS = 8, RING_BYTES = 200 * 1024;
+template <typename T, bool MIS>
+__global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const T* __restrict__ x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
+                                                                         float* __restrict__ scale, int M, int K, int slots, int slot_bytes, unsigned int* status) {
+    extern __shared__ __align__(16) unsigned char s_ring[];
+    __shared__ uint64_t s_bar[RING_WARPS * RING_MAX_SLOTS];
+    __shared__ int s_abort;
+    constexpr int VE = Chunk<T>::VE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (K + VE - 1) / VE;
+    const uint32_t bars = smem_u32(s_bar + warp * RING_MAX_SLOTS);
+    unsigned char* ring = s_ring + (size_t)warp * slots * slot_bytes;
+    if (threadIdx.x == 0) s_abort = 0;
+    if (lane == 0) {
+        for (int s = 0; s < slots; s++) mbar_init(bars + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long step = (long long)gridDim.x * RING_WARPS;
+    auto request = [&](long long m, int s) {  // lane 0
+        const uintptr_t from = (uintptr_t)(x + m * x_stride), lo = from & ~(uintptr_t)15, hi = (from + (size_t)K * sizeof(T) + 15) & ~(uintptr_t)15;
+        mbar_arrive_expect_tx(bars + 8 * s, (uint32_t)(hi - lo));
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(ring + s * slot_bytes)), "l"(lo),
+                     "r"((uint32_t)(hi - lo)), "r"(bars + 8 * s)
+                     : "memory");
+    };
+    const long long m0 = (long long)blockIdx.x * RING_WARPS + warp;
+    if (lane == 0)
+        for (int s = 0; s < slots; s++)
+            if (m0 + s * step < M) request(m0 + s * step, s);
+    __syncwarp();
+    int s = 0;
+    uint32_t ph = 0;
+    for (long long m = m0; m < M; m += step) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(bars + 8 * s, ph, &s_abort, status, 13))) {
+            // a wait gave up: give the copies already requested time to land before shared memory is released
+            for (int i = 0; i < 1000; i++) __nanosleep(1000);
+            break;
+        }
+        const T* row = reinterpret_cast<const T*>(ring + s * slot_bytes + (MIS ? (uintptr_t)(x + m * x_stride) & 15 : 0));
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int i = lane; i < chunks; i += 32) top = widen_max(top, load_chunk<T, MIS>(row, i, K));
+        const RowScale sc = row_scale(__reduce_max_sync(0xFFFFFFFFu, magnitude_bits<T>(top)), lane == 0 ? scale + m : nullptr);
+        int8_t* out = q + m * q_stride;
+#pragma unroll 2
+        for (int i = lane; i < chunks; i += 32) finish_chunk(load_chunk<T, MIS>(row, i, K), out, i, K, sc);
+        __syncwarp();
+        if (lane == 0 && m + slots * step < M) {
+            fence_async();  // the warp's reads before the copy's writes
+            request(m + slots * step, s);
+        }
+        if (++s == slots) { s = 0; ph ^= 1; }
+    }
 }
 
 template <typename... Args>
-int launch(void (*kern)(Args...), long long grid, int threads, cudaStream_t stream, Args... args) {
+int launch(void (*kern)(Args...), long long grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -229,18 +298,37 @@ int launch(void (*kern)(Args...), long long grid, int threads, cudaStream_t stre
     return TNNS_OK;
 }
 
-// The fewest threads that hold a row in four chunks each, so that many rows are on their way at once; one row by itself takes
-// more threads instead (the launch is all latency then).
+template <typename T, int GROUP, int NV, bool MIS, bool LONG = false>
+int launch_rows(const T* x, long long x_stride, int8_t* q, long long q_stride, float* scale, int M, int K, cudaStream_t st) {
+    constexpr int THREADS = GROUP < 256 ? 256 : GROUP, ROWS = THREADS / GROUP;
+    return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, GROUP, NV, MIS, LONG>, ((long long)M + ROWS - 1) / ROWS, THREADS, 0, st, x,
+                                                                             x_stride, q, q_stride, scale, M, K);
+}
+// Rows enough for every warp of the ring form to have two: that one, where its slots hold the row.  Else the fewest threads that hold a
+// row in four chunks each; a few rows by themselves take more threads (the launch is all latency then).
 template <typename T, bool MIS>
 int launch_quantise(tnns_cuda_ctx* ctx, const T* x, long long x_stride, int8_t* q, long long q_stride, float* scale, int M, int K, cudaStream_t st) {
     const int chunks = (K + Chunk<T>::VE - 1) / Chunk<T>::VE;
-    if (chunks <= 32) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 32, 1, MIS, false>, ((long long)M + 7) / 8, 256, st, x, x_stride, q, q_stride, scale, M, K);
-    if (chunks <= 128 && M > ctx->sm_count) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 32, 4, MIS, false>, ((long long)M + 7) / 8, 256, st, x, x_stride, q, q_stride, scale, M, K);
-    if (chunks <= 256) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 256, 1, MIS, false>, M, 256, st, x, x_stride, q, q_stride, scale, M, K);
-    if (chunks <= 1024 && M > ctx->sm_count) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 256, 4, MIS, false>, M, 256, st, x, x_stride, q, q_stride, scale, M, K);
-    if (chunks <= 1024) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 1024, 1, MIS, false>, M, 1024, st, x, x_stride, q, q_stride, scale, M, K);
-    if (chunks <= 4096) return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 1024, 4, MIS, false>, M, 1024, st, x, x_stride, q, q_stride, scale, M, K);
-    return launch<const T*, long long, int8_t*, long long, float*, int, int>(quantise_i8_kernel<T, 1024, 4, MIS, true>, M, 1024, st, x, x_stride, q, q_stride, scale, M, K);
+    const bool many = M > ctx->sm_count;
+    const long long slot = (((long long)K * sizeof(T) + 15) / 16 + 1) * 16;  // a row may touch one 16-byte vector more than its size
+    if (M >= 2LL * RING_WARPS * ctx->sm_count && slot * RING_WARPS <= RING_BYTES) {
+        auto kern = quantise_ring_kernel<T, MIS>;
+        static bool set[64] = {false};  // the attribute belongs to (function, device)
+        if (!set[ctx->device & 63]) {
+            TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES));
+            set[ctx->device & 63] = true;
+        }
+        const int slots = (int)std::min<long long>(RING_MAX_SLOTS, RING_BYTES / (slot * RING_WARPS));
+        return launch<const T*, long long, int8_t*, long long, float*, int, int, int, int, unsigned int*>(kern, ctx->sm_count, RING_WARPS * 32, (size_t)slots * RING_WARPS * slot, st, x,
+                                                                                                          x_stride, q, q_stride, scale, M, K, slots, (int)slot, ctx->d_status);
+    }
+    if (chunks <= 32) return launch_rows<T, 32, 1, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    if (chunks <= 128 && many) return launch_rows<T, 32, 4, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    if (chunks <= 256) return launch_rows<T, 256, 1, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    if (chunks <= 1024 && many) return launch_rows<T, 256, 4, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    if (chunks <= 1024) return launch_rows<T, 1024, 1, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    if (chunks <= 4096) return launch_rows<T, 1024, 4, MIS>(x, x_stride, q, q_stride, scale, M, K, st);
+    return launch_rows<T, 1024, 4, MIS, true>(x, x_stride, q, q_stride, scale, M, K, st);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -254,104 +342,113 @@ struct CombineArgs {
     const float* weights;
     void* out;
     long long out_stride;
-    int places, top_k, T, N, out_dtype, per_row;  // per_row: vectors of V columns
+    int places, top_k, T, N, out_dtype, per_row;  // per_row: chunks of VE columns
 };
-template <int V>
-__device__ __forceinline__ void store_vec(const CombineArgs& p, long long at, const float (&f)[V]) {
+template <int VE>
+__device__ __forceinline__ void store_sums(const CombineArgs& p, long long row, int c0, const float (&f)[VE]) {
+    const bool whole = c0 >= 0 && c0 + VE <= p.N;
     if (p.out_dtype == TNNS_F32) {
-        float* o = (float*)p.out + at;
-        if constexpr (V == 8) {
-            reinterpret_cast<float4*>(o)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            reinterpret_cast<float4*>(o)[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else if constexpr (V == 2) *reinterpret_cast<float2*>(o) = make_float2(f[0], f[1]);
-        else *o = f[0];
+        float* o = (float*)p.out + row + c0;
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < VE; j += 4) *reinterpret_cast<float4*>(o + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; j++)
+                if (c0 + j >= 0 && c0 + j < p.N) o[j] = f[j];
+        }
         return;
     }
-    uint16_t h[V];
+    uint16_t h[VE];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
+    for (int j = 0; j < VE; j++) {
         if (p.out_dtype == TNNS_F16) h[j] = __half_as_ushort(__float2half_rn(f[j]));
         else h[j] = __bfloat16_as_ushort(__float2bfloat16_rn(f[j]));
     }
-    uint16_t* o = (uint16_t*)p.out + at;
-    if constexpr (V == 8) *reinterpret_cast<uint4*>(o) = make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16);
-    else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(o) = h[0] | (uint32_t)h[1] << 16;
-    else *o = h[0];
-}
-template <typename T, int V>
-struct RawVec {
-    uint32_t w[V * sizeof(T) <= 4 ? 1 : V * sizeof(T) / 4];
-};
-template <typename T, int V>
-__device__ __forceinline__ RawVec<T, V> load_vec(const T* at) {
-    RawVec<T, V> r;
-    constexpr int B = V * sizeof(T);
-    if constexpr (B >= 16) {
+    uint16_t* o = (uint16_t*)p.out + row + c0;
+    if (whole) {
+        uint32_t w[VE / 2];
 #pragma unroll
-        for (int i = 0; i < B / 16; i++) {
-            const uint4 v = reinterpret_cast<const uint4*>(at)[i];
-            r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
-        }
-    } else if constexpr (B == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(at);
-        r.w[0] = v.x; r.w[1] = v.y;
-    } else if constexpr (B == 4) r.w[0] = *reinterpret_cast<const uint32_t*>(at);
-    else r.w[0] = *reinterpret_cast<const uint16_t*>(at);
-    return r;
-}
-template <typename T, int V>
-__device__ __forceinline__ void add_vec(const RawVec<T, V>& r, float w, float (&sum)[V]) {
+        for (int j = 0; j < VE / 2; j++) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+        if constexpr (VE == 8) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        float v;
-        if constexpr (sizeof(T) == 4) v = __uint_as_float(r.w[j]);
-        else {
-            const unsigned short h = (unsigned short)(r.w[j >> 1] >> (16 * (j & 1)));
-            if constexpr (sizeof(T) == 2) v = to_f32(*reinterpret_cast<const T*>(&h));
-        }
-        sum[j] = fmaf(w, v, sum[j]);
+        for (int j = 0; j < VE; j++)
+            if (c0 + j >= 0 && c0 + j < p.N) o[j] = h[j];
     }
 }
 
-// One thread V neighbouring columns of a token, the rows of eight slots on their way at once.  Bounded by memory: every row of y is
-// read once, V * 32 neighbouring columns a warp.
-template <typename T, int V>
+// One thread a chunk of VE neighbouring columns (16 bytes of y) of a token, the rows of eight slots on their way at once.  Bounded by
+// memory: every row of y is read once.  MIS: rows need not start on 16 bytes; the first chunk of a row begins where its results are
+// aligned (at a column up to VE - 1 below 0), and y is fetched as the aligned vectors that hold the chunk.
+template <typename T, bool MIS>
 __global__ void __launch_bounds__(256) combine_kernel(CombineArgs p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int U = 8;
+    constexpr int U = 8, VE = Chunk<T>::VE;
     const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
     if (item >= (long long)p.T * p.per_row) return;
     const int t = item < 0xFFFFFFFFLL ? (int)((uint32_t)item / (uint32_t)p.per_row) : (int)(item / p.per_row);
-    const int n = (int)(item - (long long)t * p.per_row) * V;
+    const long long out_row = (long long)t * p.out_stride;
+    int c0 = (int)(item - (long long)t * p.per_row) * VE;
+    if (MIS) {
+        const uintptr_t elements = ((uintptr_t)p.out >> (p.out_dtype == TNNS_F32 ? 2 : 1)) + (uintptr_t)out_row;
+        c0 -= (int)(elements % VE);
+        if (c0 >= p.N) return;
+    }
     const int32_t* slots = p.slots + (long long)t * p.top_k;
     const float* weights = p.weights + (long long)t * p.top_k;
-    const T* y = (const T*)p.y + n;
-    float sum[V] = {};
+    float sum[VE] = {};
     for (int j0 = 0; j0 < p.top_k; j0 += U) {
         int at[U];
         float w[U];
-        RawVec<T, V> r[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             at[u] = j0 + u < p.top_k ? __ldg(slots + j0 + u) : -1;
             w[u] = j0 + u < p.top_k ? __ldg(weights + j0 + u) : 0.f;
         }
+        uint4 a[U], b[MIS ? U : 1];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] = make_uint4(0, 0, 0, 0);
+            if (MIS) b[u] = make_uint4(0, 0, 0, 0);
+            if (at[u] >= 0 && at[u] < p.places) {
+                const T* row = (const T*)p.y + (long long)at[u] * p.y_stride;
+                if (!MIS) a[u] = *reinterpret_cast<const uint4*>(row + c0);
+                else {
+                    // of the two aligned vectors those that hold elements of the row
+                    const uintptr_t from = (uintptr_t)(row + c0), lo = from & ~(uintptr_t)15;
+                    if (lo + 16 > (uintptr_t)row) a[u] = *reinterpret_cast<const uint4*>(lo);
+                    if (from != lo && lo + 16 < (uintptr_t)(row + min(c0 + VE, p.N))) b[u] = *reinterpret_cast<const uint4*>(lo + 16);
+                }
+            }
+        }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (at[u] >= 0 && at[u] < p.places) r[u] = load_vec<T, V>(y + (long long)at[u] * p.y_stride);
+            if (at[u] >= 0 && at[u] < p.places) {
+                Chunk<T> c;
+                float f[VE];
+                if (MIS) realign<T>(a[u], b[u], (int)((uintptr_t)((const T*)p.y + (long long)at[u] * p.y_stride + c0) & 15), c.w);
+                else { c.w[0] = a[u].x; c.w[1] = a[u].y; c.w[2] = a[u].z; c.w[3] = a[u].w; }
+                unpack(c, f);
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            if (at[u] >= 0 && at[u] < p.places) add_vec<T, V>(r[u], w[u], sum);
+                for (int j = 0; j < VE; j++) sum[j] = fmaf(w[u], f[j], sum[j]);
+            }
     }
-    store_vec<V>(p, (long long)t * p.out_stride + n, sum);
+    store_sums<VE>(p, out_row, c0, sum);
 }
 
-template <typename T, int V>
-int launch_combine(const CombineArgs& a, cudaStream_t st) {
+template <typename T>
+int launch_combine(CombineArgs a, cudaStream_t st) {
+    constexpr int VE = Chunk<T>::VE;
+    const int bo = tnns_dtype_bytes(a.out_dtype);
+    const bool mis = a.N % VE || ((uintptr_t)a.y | (uintptr_t)(a.y_stride * (long long)sizeof(T))) % 16 || ((uintptr_t)a.out | (uintptr_t)(a.out_stride * bo)) % (VE * bo);
+    a.per_row = mis ? (int)(((long long)a.N + 2 * VE - 2) / VE) : a.N / VE;
     const long long blocks = ((long long)a.T * a.per_row + 255) / 256;
-    if (blocks > 0x7FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "%d tokens of %d columns", a.T, a.N);
-    return launch<CombineArgs>(combine_kernel<T, V>, blocks, 256, st, a);
+    if (blocks > 0x7FFFFFFFLL || a.N > 0x7FFFFF00) return tnns_fail(TNNS_ERR_UNSUPPORTED, "%d tokens of %d columns", a.T, a.N);
+    if (mis) return launch<CombineArgs>(combine_kernel<T, true>, blocks, 256, 0, st, a);
+    return launch<CombineArgs>(combine_kernel<T, false>, blocks, 256, 0, st, a);
 }
 
 }  // namespace
@@ -389,16 +486,9 @@ int tnns_cuda_combine(tnns_cuda_ctx* ctx, const void* d_y, int dtype, long long 
     CombineArgs a;
     a.y = d_y; a.y_stride = y_stride; a.slots = d_slots; a.weights = d_weights; a.out = d_out; a.out_stride = out_stride;
     a.places = places; a.top_k = top_k; a.T = T; a.N = N; a.out_dtype = out_dtype;
-    // columns of a thread: as many as rows and bases allow to move at once (8 elements: 16 or 32 bytes)
-    const int bi = tnns_dtype_bytes(dtype), bo = tnns_dtype_bytes(out_dtype);
-    auto fits = [&](int v) {
-        const int ai = std::min(16, v * bi), ao = std::min(16, v * bo);
-        return N % v == 0 && ((uintptr_t)d_y | (uintptr_t)(y_stride * bi)) % ai == 0 && ((uintptr_t)d_out | (uintptr_t)(out_stride * bo)) % ao == 0;
-    };
-    const int v = fits(8) ? 8 : fits(2) ? 2 : 1;
-    a.per_row = N / v;
+    a.per_row = 0;
     const cudaStream_t st = (cudaStream_t)stream;
-    TNNS_FOR_DTYPE(dtype, TI, return v == 8 ? (launch_combine<TI, 8>(a, st)) : v == 2 ? (launch_combine<TI, 2>(a, st)) : (launch_combine<TI, 1>(a, st)));
+    TNNS_FOR_DTYPE(dtype, TI, return launch_combine<TI>(a, st));
 }
 
 }  // extern "C"

@@ -53,7 +53,8 @@ def run_quantise(ctx, x, x_stride=None, q_stride=None, shift=0):
 @pytest.mark.parametrize("M,K,x_stride,q_stride,shift", [
     (1, 1, None, None, 0), (1, 64, None, None, 0), (3, 65, 67, 80, 1), (5, 127, None, None, 0), (2, 1024, None, None, 0), (7, 1000, 1003, 1024, 3),
     (300, 129, None, None, 0), (33, 4096, None, None, 0), (2, 5000, None, None, 0), (1, 16384, None, None, 0), (9, 16385, 16400, 16416, 0), (2, 50001, None, None, 1),
-    (5000, 72, None, None, 0), (1200, 2048, 2056, 2064, 8)], ids=str)
+    (5000, 72, None, None, 0), (1200, 2048, 2056, 2064, 8), (4000, 1, None, None, 0), (3601, 1000, 1003, 1024, 1), (3600, 4097, 4099, 4112, 3), (9000, 512, 520, None, 8),
+    (3700, 8192, None, None, 0), (7200, 40, 41, None, 0)], ids=str)
 def test_quantise(M, K, x_stride, q_stride, shift, dtype, gpu_ctx):
     x = (torch.randn(M, K, generator=gen(M * 131 + K)) * torch.exp(torch.randn(M, 1, generator=gen(K)) * 4)).to(DT[dtype])
     q, s = run_quantise(gpu_ctx, x, x_stride, q_stride, shift)
@@ -82,8 +83,9 @@ def test_quantise_halves(K, dtype, gpu_ctx):
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("K", [40, 1536, 20001])
-def test_quantise_special_rows(K, dtype, gpu_ctx):
+@pytest.mark.parametrize("times", [1, 400])
+@pytest.mark.parametrize("K", [40, 1536, 2049, 20001])
+def test_quantise_special_rows(K, times, dtype, gpu_ctx):
     """Zeros, negative zeros, one value, infinities, NaN, the type's largest and smallest numbers."""
     top, small = torch.finfo(DT[dtype]).max, {"f32": 2.0 ** -149, "f16": 2.0 ** -24, "bf16": 2.0 ** -133}[dtype]
     x = torch.randn(11, K, generator=gen(K)).to(DT[dtype])
@@ -100,6 +102,7 @@ def test_quantise_special_rows(K, dtype, gpu_ctx):
     x[9] = 0
     x[9, 3], x[9, 4] = 5 * small, 2 * small
     x[10, 0], x[10, 1] = float("nan"), float("inf")
+    x = x.repeat(times if K < 10000 else 1, 1)
     q, s = run_quantise(gpu_ctx, x)
     want_q, want_s = quantise(x)
     assert np.array_equal(q, want_q) and np.array_equal(s, want_s, equal_nan=True)
@@ -307,7 +310,8 @@ COUNTS = [
     ([1], 64, 32), ([0, 3, 0, 1], 100, 50), ([8] * 8, 256, 256), ([0] * 5 + [9], 130, 96), ([17, 0, 33, 5, 64], 512, 200), ([1, 2, 3, 0, 0, 7, 130], 300, 129),
     ([128, 129, 127, 1], 384, 256), ([300, 0, 12, 500], 640, 520), ([5] * 150, 96, 130), ([1000, 3, 1, 700], 1024, 264), ([2] * 300 + [0] * 20, 64, 70),
     ([2000], 256, 513), ([40] * 30, 1100, 257), ([16] * 20 + [1], 777, 1000), ([3000, 2500], 500, 1300),
-    ([700, 1, 900, 0, 257, 256, 255, 1400], 640, 2100)]
+    ([700, 1, 900, 0, 257, 256, 255, 1400], 640, 2100),
+    ([130] * 60, 2048, 1024), ([60] * 40, 4000, 200), ([90] * 6, 6000, 300)]
 
 
 @pytest.mark.parametrize("gather", [True, False])

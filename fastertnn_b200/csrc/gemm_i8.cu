@@ -235,16 +235,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Ar
 
 // Stages of 128 bytes of K: 128 rows of q (one tensor copy, or 16-byte copies by the gather warps where places name their rows) and
 // BN / CG channels of weights (contiguous copies of the tiled image).
-template <int BN, int CG>
+template <int BN, int CG, bool GATHER>
 struct TcI8 {
     static constexpr int A_STAGE = BM * KCH, B_STAGE = BN / CG * KCH, STAGE = A_STAGE + B_STAGE;
     static constexpr int NSTG = 5 * 32768 / STAGE;
     static constexpr int NBUF = 2;  // accumulator sets
     static constexpr int COLS = NBUF * BN < 32 ? 32 : NBUF * BN;
-    static constexpr int GATHER0 = 2, GATHER_WARPS = 6, EPI0 = GATHER0 + GATHER_WARPS, EPI_WARPS = 8, THREADS = 32 * (EPI0 + EPI_WARPS);
+    static constexpr int GATHER0 = 2, GATHER_WARPS = GATHER ? 6 : 2, EPI0 = GATHER0 + GATHER_WARPS;  // (EPI0: a multiple of four)
+    static constexpr int EPI_WARPS = BN == 64 ? 8 : 16, HN = BN / (EPI_WARPS / 4), THREADS = 32 * (EPI0 + EPI_WARPS);  // HN: channels of an epilogue warp
     static constexpr int BARS = 2 * NSTG + 2 * NBUF;
-    static constexpr int STAGED = 32;  // words of a row of a warp's buffer for results on their way out
-    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + EPI_WARPS * (32 * STAGED + BN / 2) * 4 + list_bytes(experts); }
+    static constexpr int STAGED = 16;  // words of a row of a warp's buffer for results on their way out
+    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + EPI_WARPS * (32 * STAGED + HN) * 4 + list_bytes(experts); }
+    static_assert(!GATHER || NSTG <= GATHER_WARPS, "a gather warp for every slot");
 };
 struct alignas(64) MapsI8 {
     CUtensorMap q, w;
@@ -283,34 +285,48 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
-// A warp's results leave through a buffer of 32 rows x 128 bytes in shared memory, so that it writes whole lines along the rows of
-// y: the 16-byte pieces of a row lie in the pattern piece ^ (row % 8), which keeps both directions free of bank conflicts.
-__device__ __forceinline__ uint32_t* staged(uint32_t* stage, int row, int word) { return stage + row * 32 + ((((word >> 2) ^ row) & 7) << 2) + (word & 3); }
-
-// Rows 0 .. rows - 1 of the buffer to `y`, `step` bytes from row to row; `have` bytes of each exist (a multiple of `size`, an element's
-// bytes).  vec: bytes that may be stored at once everywhere in y.
-__device__ __forceinline__ void store_rows(uint32_t* stage, unsigned char* y, long long step, int rows, int have, int vec, int size, int lane) {
-    if (vec >= 16 && have % 16 == 0) {
-        unsigned char* at = y + (lane >> 3) * step + (lane & 7) * 16;
+__device__ __forceinline__ void store_32b(unsigned char* at, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// 64 bytes of each of a warp's rows to `y` (the first row's), `step` bytes from row to row: w = those of the lane's row; `have` bytes of
+// a row exist (a multiple of `size`, an element's bytes).  vec: bytes that may be stored at once everywhere in y.  Whole 64 bytes go
+// straight from the lanes where rows allow 16 bytes at once.  The rest passes through the warp's 32 x 64 bytes of shared memory, so
+// that the warp writes along the rows; the 16-byte pieces of a row lie in the pattern piece ^ (row / 2) % 4, free of bank conflicts.
+__device__ __forceinline__ void store_rows(const uint32_t* w, uint32_t* stage, unsigned char* y, long long step, int rows, int have, int vec, int size, int lane) {
+    if (vec >= 16 && have == 64) {
+        if (lane >= rows) return;
+        unsigned char* at = y + lane * step;
+        if (vec >= 32) {
+            store_32b(at, w);
+            store_32b(at + 32, w + 8);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++, at += 4 * step) {
-            const int r = 4 * i + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4*>(staged(stage, r, 4 * (lane & 7)));
-            if (r < rows && 16 * (lane & 7) < have) *reinterpret_cast<uint4*>(at) = v;
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
         }
-    } else {
-        for (int r = 0; r < rows; r++, y += step) {
-            const uint32_t v = *staged(stage, r, lane);
-            if (size == 4 || (reinterpret_cast<uintptr_t>(y) & 2) == 0) {
-                if (4 * lane + 4 <= have) *reinterpret_cast<uint32_t*>(y + 4 * lane) = v;
-                else if (4 * lane + 2 <= have) *reinterpret_cast<uint16_t*>(y + 4 * lane) = (uint16_t)v;
-            } else {
-                // a row that starts between two words: the halves of neighbours together, the first and the last by themselves
-                const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
-                if (lane == 0) *reinterpret_cast<uint16_t*>(y) = (uint16_t)v;
-                if (4 * lane + 6 <= have) *reinterpret_cast<uint32_t*>(y + 2 + 4 * lane) = __funnelshift_r(v, next, 16);
-                else if (4 * lane + 4 <= have) *reinterpret_cast<uint16_t*>(y + 2 + 4 * lane) = (uint16_t)(v >> 16);
-            }
+        return;
+    }
+    auto at = [&](int row, int word) { return stage + row * 16 + ((((word >> 2) ^ (row >> 1)) & 3) << 2) + (word & 3); };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(at(lane, i)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    __syncwarp();
+    // half a warp a row
+    const int col = lane & 15;
+    y += (lane >> 4) * step;
+    for (int r0 = 0; r0 < rows; r0 += 2, y += 2 * step) {
+        const int r = r0 + (lane >> 4);
+        const uint32_t v = *at(r, col), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+        if (r >= rows) continue;
+        if (size == 4 || (reinterpret_cast<uintptr_t>(y) & 2) == 0) {
+            if (4 * col + 4 <= have) *reinterpret_cast<uint32_t*>(y + 4 * col) = v;
+            else if (4 * col + 2 <= have) *reinterpret_cast<uint16_t*>(y + 4 * col) = (uint16_t)v;
+        } else {
+            // a row that starts between two words: the halves of neighbours together, the first and the last by themselves
+            if (col == 0) *reinterpret_cast<uint16_t*>(y) = (uint16_t)v;
+            if (4 * col + 6 <= have) *reinterpret_cast<uint32_t*>(y + 2 + 4 * col) = __funnelshift_r(v, next, 16);
+            else if (4 * col + 4 <= have) *reinterpret_cast<uint16_t*>(y + 2 + 4 * col) = (uint16_t)(v >> 16);
         }
     }
 }
@@ -333,36 +349,27 @@ __device__ __forceinline__ float2 finish_pair(uint32_t a0, uint32_t a1, float rs
     }
     return f;
 }
-// 32 accumulators of the lane's row -> bytes of the buffer's row from word w0 on.
-__device__ __forceinline__ void finish_chunk(int dtype, const uint32_t (&v)[32], float rs, const float* ws, float alpha, int mode, uint32_t* stage, int lane, int w0) {
-    if (dtype == TNNS_F32) {
+// C accumulators of the lane's row (64 bytes of results) -> words.
+template <int C>
+__device__ __forceinline__ void finish_words(int dtype, const uint32_t* v, float rs, const float* ws, float alpha, int mode, uint32_t (&w)[16]) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 w4 = *reinterpret_cast<const float4*>(ws + j);
-            const float2 a = finish_pair(v[j], v[j + 1], rs, make_float2(w4.x, w4.y), alpha, mode), b = finish_pair(v[j + 2], v[j + 3], rs, make_float2(w4.z, w4.w), alpha, mode);
-            *reinterpret_cast<float4*>(staged(stage, lane, j)) = make_float4(a.x, a.y, b.x, b.y);
+    for (int j = 0; j < C; j += 4) {
+        const float4 w4 = *reinterpret_cast<const float4*>(ws + j);
+        const float2 a = finish_pair(v[j], v[j + 1], rs, make_float2(w4.x, w4.y), alpha, mode), b = finish_pair(v[j + 2], v[j + 3], rs, make_float2(w4.z, w4.w), alpha, mode);
+        if (C == 16) {
+            w[j] = __float_as_uint(a.x);
+            w[(j + 1) % 16] = __float_as_uint(a.y);
+            w[(j + 2) % 16] = __float_as_uint(b.x);
+            w[(j + 3) % 16] = __float_as_uint(b.y);
+        } else if (dtype == TNNS_F16) {
+            const __half2 x = __floats2half2_rn(a.x, a.y), y = __floats2half2_rn(b.x, b.y);
+            w[j / 2] = *reinterpret_cast<const uint32_t*>(&x);
+            w[j / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y);
+        } else {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(a.x, a.y), y = __floats2bfloat162_rn(b.x, b.y);
+            w[j / 2] = *reinterpret_cast<const uint32_t*>(&x);
+            w[j / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            const float4 w4 = *reinterpret_cast<const float4*>(ws + j + 2 * i);
-            const float2 a = finish_pair(v[j + 2 * i], v[j + 2 * i + 1], rs, make_float2(w4.x, w4.y), alpha, mode);
-            const float2 b = finish_pair(v[j + 2 * i + 2], v[j + 2 * i + 3], rs, make_float2(w4.z, w4.w), alpha, mode);
-            if (dtype == TNNS_F16) {
-                const __half2 x = __floats2half2_rn(a.x, a.y), y = __floats2half2_rn(b.x, b.y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&x);
-                w[i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-            } else {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(a.x, a.y), y = __floats2bfloat162_rn(b.x, b.y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&x);
-                w[i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-            }
-        }
-        *reinterpret_cast<uint4*>(staged(stage, lane, w0 + (j >> 1))) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -376,9 +383,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // MMAs, warps 2 to 7 gather rows where places name them (each a slot of the ring, so that all are on their way at once), warps 8 to 15
 // scale, round and store one accumulator while the MMAs fill the other.  Gathering through the copy engine, four rows a request,
 // was measured first: 80 clocks a request of 512 bytes, 360 us where the warps take X (8192 tokens, 8 of 64 experts, 2048 -> 1024).
-template <int BN, int CG>
-__global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(GemmI8Args p, const __grid_constant__ MapsI8 maps) {
-    using Cfg = TcI8<BN, CG>;
+template <int BN, int CG, bool GATHER>
+__global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_kernel(const __grid_constant__ GemmI8Args p, const __grid_constant__ MapsI8 maps) {
+    using Cfg = TcI8<BN, CG, GATHER>;
     constexpr int NSTG = Cfg::NSTG, NBUF = Cfg::NBUF, TM = CG * BM;
     // s32 accumulators, signed 8-bit operands, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
     constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
@@ -390,8 +397,8 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* s_stage = tmem_slot + 4;                                                      // [epilogue warp][32][STAGED]
-    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][BN / 2]: its channels' scales
-    int2* s_range = reinterpret_cast<int2*>(s_ws + Cfg::EPI_WARPS * (BN / 2));
+    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][HN]: its channels' scales
+    int2* s_range = reinterpret_cast<int2*>(s_ws + Cfg::EPI_WARPS * Cfg::HN);
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
@@ -399,7 +406,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
 
     if (tid == 0) {
         for (int s = 0; s < NSTG; s++) {
-            mbar_init(bar_full + 8 * s, p.rows ? 1 + CG : 1);  // the copies' bytes, and a gather warp of each block
+            mbar_init(bar_full + 8 * s, GATHER ? 1 + CG : 1);  // the copies' bytes, and a gather warp of each block
             mbar_init(bar_empty + 8 * s, 1);
         }
         for (int b = 0; b < NBUF; b++) {
@@ -455,7 +462,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
     const uint32_t full_lead = CG == 2 ? mapa_shared(bar_full, 0) : bar_full;
     if (warp == WARP_TMA) {
         if (lane == 0) {
-            const uint32_t bytes = CG * (p.rows ? Cfg::B_STAGE : Cfg::STAGE);
+            const uint32_t bytes = CG * (GATHER ? Cfg::B_STAGE : Cfg::STAGE);
             uint32_t s = 0, ph = 1;
             for (int t = unit; t < tiles; t += units) {
                 const Tile c = tile_at(t);
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
                         if (CG == 2) tma_tile2d_g2s_pair(b_dst + n * KCH, &maps.w, 0, (int)(tile * WT + nn % WT), bar);
                         else bulk_g2s(b_dst + n * KCH, p.img + tile * WT_BYTES + (nn % WT) * KCH, HIGH * KCH, bar);
                     }
-                    if (!p.rows) {
+                    if (!GATHER) {
                         if (CG == 2) tma_tile2d_g2s_pair(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
                         else tma_tile2d_g2s(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
                     }
@@ -512,12 +519,11 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
             }
         }
     } else if (warp < Cfg::EPI0) {
-        if (p.rows) {
+        if (GATHER) {
             // Stage i of the block's sequence belongs to gather warp i % NSTG, and so does its slot of the ring: a warp's successive waits on a
             // slot's barrier are then successive phases, which is all that a parity tells apart.  (Six warps on five slots met a slot again
             // one lap early and wrote over a stage that was still to be read; the launch failed.)
             constexpr int GW = NSTG;
-            static_assert(GW <= Cfg::GATHER_WARPS, "a gather warp for every slot");
             const int own = warp - Cfg::GATHER0;
             uint32_t first = 0;  // stages of the tiles before this one, modulo GW and modulo 2 * NSTG
             uint32_t slot0 = 0;
@@ -553,8 +559,8 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - Cfg::EPI0) >> 2;
-        constexpr int HN = BN / 2, NC = HN / 32;  // channels of the half, in chunks of 32
+        const int q = warp & 3, part = (warp - Cfg::EPI0) >> 2;
+        constexpr int HN = Cfg::HN, NC = HN / 32;  // channels of the part, in chunks of 32
         const uint32_t tempty_lead = CG == 2 ? mapa_shared(bar_tempty, 0) : bar_tempty;
         uint32_t* stage = s_stage + (warp - Cfg::EPI0) * 32 * Cfg::STAGED;
         const int mode = p.alpha == 1.0f ? 0 : p.alpha > 0.0f && p.alpha < 1.0f ? 1 : 2;
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
         float* wsc = s_ws + (warp - Cfg::EPI0) * HN;
         auto fetch = [&](int t) {
             c = tile_at(t);
-            const int place = c.m0 + (int)rank * BM + q * 32 + lane, n = c.n * BN + half * HN + lane;
+            const int place = c.m0 + (int)rank * BM + q * 32 + lane, n = c.n * BN + part * HN + lane;
             row = place < c.last ? row_of(p, place) : -1;
 #pragma unroll
             for (int i = 0; i < NC; i++) ws[i] = n + 32 * i < p.N ? __ldg(p.w_scale + (long long)c.e * p.n_tiles * WT + n + 32 * i) : 0.f;
@@ -587,19 +593,16 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
             if (!warp_wait(bar_tfull + 8 * buf, (lt / NBUF) & 1, abort_flag, p.status, 4)) goto done;
             tc_fence_after();
             if (t + units < tiles) fetch(t + units);
-            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + half * HN;
-            const int n0 = now.n * BN + half * HN, size = p.dtype == TNNS_F32 ? 4 : 2;
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * HN;
+            const int n0 = now.n * BN + part * HN, size = p.dtype == TNNS_F32 ? 4 : 2;
             unsigned char* y0 = (unsigned char*)p.y + ((long long)place0 * p.y_stride + n0) * size;
             const long long step = p.y_stride * size;
-            // a pass: as many channels as two loads of 32, and 128 bytes of every row (fp32: twice)
-            constexpr int CH = NC < 2 ? 1 : 2;
-#pragma unroll
-            for (int i = 0; i < NC; i += CH) {
-                uint32_t v[CH][32];
-#pragma unroll
-                for (int h = 0; h < CH; h++) tmem_ld_32(taddr + 32 * (i + h), v[h]);
+#pragma unroll 1
+            for (int i = 0; i < NC; i++) {
+                uint32_t v[32];
+                tmem_ld_32(taddr + 32 * i, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (i + CH >= NC) {  // the last columns are in registers: the accumulator may be written again
+                if (i + 1 == NC) {  // the last columns are in registers: the accumulator may be written again
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -607,19 +610,23 @@ __global__ void __launch_bounds__(TcI8<BN, CG>::THREADS, 1) gemm_i8_tc_kernel(Ge
                     }
                 }
                 if (i == 0) rs = row >= 0 ? p.scale[row] : 0.f;  // the next tile's
-                if (rows_here > 0 && n0 + 32 * i < p.N) {
-#pragma unroll
-                    for (int h = 0; h < CH; h++) {
-                        finish_chunk(p.dtype, v[h], rs_now, wsc + 32 * (i + h), p.alpha, mode, stage, lane, 16 * h);
-                        if (size == 4 || h + 1 == CH) {
-                            const int first = size == 4 ? i + h : i;  // of the chunks in the buffer
-                            const int have = min(p.N - n0 - 32 * first, size == 4 ? 32 : 32 * CH) * size;
-                            __syncwarp();
-                            if (have > 0) store_rows(stage, y0 + 32 * first * size, step, rows_here, have, p.y_vec, size, lane);
-                            __syncwarp();
+                const int have = (p.N - n0 - 32 * i) * size;
+                if (rows_here > 0 && have > 0) {
+                    uint32_t w[16];
+                    unsigned char* y = y0 + 32 * i * size;
+                    if (size == 4) {
+                        finish_words<16>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
+                        store_rows(w, stage, y, step, rows_here, min(have, 64), p.y_vec, 4, lane);
+                        if (have > 64) {
+                            finish_words<16>(p.dtype, v + 16, rs_now, wsc + 32 * i + 16, p.alpha, mode, w);
+                            store_rows(w, stage, y + 64, step, rows_here, min(have - 64, 64), p.y_vec, 4, lane);
                         }
+                    } else {
+                        finish_words<32>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
+                        store_rows(w, stage, y, step, rows_here, min(have, 64), p.y_vec, 2, lane);
                     }
                 }
+                __syncwarp();
             }
         }
     }
@@ -664,15 +671,15 @@ int launch(void (*kern)(Args...), tnns_cuda_ctx* ctx, int grid, int threads, siz
     return TNNS_OK;
 }
 
-template <int BN, int CG>
+template <int BN, int CG, bool GATHER>
 int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
-    using Cfg = TcI8<BN, CG>;
+    using Cfg = TcI8<BN, CG, GATHER>;
     MapsI8 maps = {};
     int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, BM, 128);
     if (rc) return rc;
     // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
     if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;
-    auto kern = gemm_i8_tc_kernel<BN, CG>;
+    auto kern = gemm_i8_tc_kernel<BN, CG, GATHER>;
     static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
     if (!smem_set[ctx->device & 63]) {
         TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::smem(MAX_EXPERTS)));
@@ -725,9 +732,9 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     if (q_rows == 0 || rows <= 8) return launch_few<1>(ctx, a, st);
     if (rows <= 16) return launch_few<2>(ctx, a, st);
     const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
-    if (tiles >= ctx->sm_count / 2) return launch_tc<256, 2>(ctx, a, st);
-    if (tiles * 4 >= ctx->sm_count) return launch_tc<128, 1>(ctx, a, st);
-    return launch_tc<64, 1>(ctx, a, st);
+    if (tiles >= ctx->sm_count / 2) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
+    if (tiles * 4 >= ctx->sm_count) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
+    return d_rows ? launch_tc<64, 1, true>(ctx, a, st) : launch_tc<64, 1, false>(ctx, a, st);
 }
 
 }  // namespace

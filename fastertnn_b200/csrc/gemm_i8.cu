@@ -124,19 +124,19 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 }
 
 // 8 * NT places x 16 channels a warp, or S warps that share the K tiles and add up their sums in shared memory; a block holds 8 / S
-// such pieces side by side.  Bounded by the weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and
-// g + 8, so four instructions multiply a whole K tile of 2 KB and no byte passes through shared memory.  The order of K within the
-// tile is the same for weights and rows.
+// such pieces side by side and goes on to others, whose weights it requests before it finishes the present ones.  Bounded by the
+// weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and g + 8, so four instructions multiply a
+// whole K tile of 2 KB and no byte passes through shared memory.  The order of K within the tile is the same for weights and rows.
 template <int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Args p, int S) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int S) {
     constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
     extern __shared__ int2 s_range[];
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int ks = warp & (S - 1), wide = FEW_WARPS / S * 16;  // this warp's part of K, channels of a block
+    const int ks = warp & (S - 1), wide = FEW_WARPS / S * 16, n_mine = (warp / S) * 16;  // this warp's part of K, channels of a block, the warp's among them
     const int n_blocks = (p.N + wide - 1) / wide;
-    const int8_t* wt;
+    const int8_t* wt = nullptr;
     uint4 a[U][4];
     auto load_weights = [&](int kt0) {
 #pragma unroll
@@ -149,38 +149,48 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Ar
                 a[u][3] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + (((t + 4) ^ g) << 4)));
             }
     };
-    auto weights_at = [&](int e, int n) { wt = p.img + ((long long)e * p.n_tiles + n / WT) * p.k_tiles * WT_BYTES + (n % WT + g) * 128; };
+    // the warp's first weights of channels n .. of expert e
+    auto begin = [&](int e, int n) {
+        if (n >= p.N) return;
+        wt = p.img + ((long long)e * p.n_tiles + n / WT) * p.k_tiles * WT_BYTES + (n % WT + g) * 128;
+        load_weights(ks);
+    };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int n_mine = (warp / S) * 16;
-    bool loaded = false;
-    if (!p.offsets) {  // one kernel: the weights' way from memory may start before the launch in front has ended
-        const int n = (int)(blockIdx.x % (unsigned)n_blocks) * wide + n_mine;
-        if (n < p.N) {
-            weights_at(0, n);
-            load_weights(ks);
-        }
-        loaded = true;
-    }
+    // one kernel: the weights' way from memory starts before the launch in front has ended
+    if (!p.offsets) begin(0, (int)(blockIdx.x % (unsigned)n_blocks) * wide + n_mine);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     list_blocks<8 * NT>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, FEW_WARPS * 32);
     const int items = s_first[p.experts] * n_blocks;
-    for (int item = blockIdx.x; item < items; item += gridDim.x, loaded = false) {
-        const int b = item / n_blocks, nb = (item - b * n_blocks) * wide, n0 = nb + n_mine;
-        const int e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
-        int acc[NT][4] = {};
-        const int2 range = s_range[e];
-        const int m0 = range.x + (b - s_first[e]) * 8 * NT;
-        if (n0 < p.N) {
-            if (!loaded) {
-                weights_at(e, n0);
-                load_weights(ks);
-            }
-            const int8_t* row[NT];
+    struct Item {
+        int e, m0, last, n0;  // expert, first place, end of the expert's places, first channel of the block
+    };
+    auto item_at = [&](int item) {
+        Item r;
+        const int b = item / n_blocks;
+        r.n0 = (item - b * n_blocks) * wide;
+        r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
+        const int2 range = s_range[r.e];
+        r.m0 = range.x + (b - s_first[r.e]) * 8 * NT;
+        r.last = range.y;
+        return r;
+    };
+    int row[NT];  // of q, that the lane's places read; -1: none
+    auto rows_at = [&](const Item& c) {
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const int place = m0 + i * 8 + g, r = place < range.y ? row_of(p, place) : -1;
-                row[i] = r >= 0 ? p.q + (long long)r * p.q_stride : nullptr;
-            }
+        for (int i = 0; i < NT; i++) {
+            const int place = c.m0 + i * 8 + g;
+            row[i] = place < c.last ? row_of(p, place) : -1;
+        }
+    };
+    Item c = {};
+    if ((int)blockIdx.x < items) {
+        c = item_at(blockIdx.x);
+        rows_at(c);
+        if (p.offsets) begin(c.e, c.n0 + n_mine);
+    }
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        int acc[NT][4] = {};
+        if (c.n0 + n_mine < p.N) {
             for (int kt0 = ks; kt0 < p.k_tiles; kt0 += S * U) {
                 uint4 x[U][NT][2];
 #pragma unroll
@@ -190,7 +200,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Ar
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const int k = (kt0 + u * S) * WT + (t + 4 * h) * 16;
-                            x[u][i][h] = row[i] && k < p.K ? load_piece(row[i], k, p.K) : make_uint4(0, 0, 0, 0);
+                            x[u][i][h] = row[i] >= 0 && k < p.K ? load_piece(p.q + (long long)row[i] * p.q_stride, k, p.K) : make_uint4(0, 0, 0, 0);
                         }
 #pragma unroll
                 for (int u = 0; u < U; u++)
@@ -206,6 +216,12 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Ar
                 load_weights(kt0 + S * U);
             }
         }
+        const Item now = c;
+        if (item + (int)gridDim.x < items) {
+            c = item_at(item + gridDim.x);
+            rows_at(c);
+            begin(c.e, c.n0 + n_mine);
+        }
         // d[0], d[1]: channel g, places 2t, 2t + 1; d[2], d[3]: channel g + 8
 #pragma unroll
         for (int i = 0; i < NT; i++)
@@ -214,12 +230,12 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(GemmI8Ar
         __syncthreads();
         // a result for each place and channel of the block, channels side by side
         for (int o = tid; o < 8 * NT * wide; o += FEW_WARPS * 32) {
-            const int c = o % wide, pl = o / wide, place = m0 + pl, n = nb + c;
-            if (place >= range.y || n >= p.N) continue;
+            const int ch = o % wide, pl = o / wide, place = now.m0 + pl, n = now.n0 + ch;
+            if (place >= now.last || n >= p.N) continue;
             int sum = 0;
-            for (int w = 0; w < S; w++) sum += s_sum[(c >> 4) * S + w][pl >> 3][(pl & 7) * 16 + (c & 15)];
+            for (int w = 0; w < S; w++) sum += s_sum[(ch >> 4) * S + w][pl >> 3][(pl & 7) * 16 + (ch & 15)];
             const int r = row_of(p, place);
-            const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)e * p.n_tiles * WT + n], p.alpha);
+            const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)now.e * p.n_tiles * WT + n], p.alpha);
             const long long at = (long long)place * p.y_stride + n;
             if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
             else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
@@ -249,7 +265,7 @@ struct TcI8 {
     static_assert(!GATHER || NSTG <= GATHER_WARPS, "a gather warp for every slot");
 };
 struct alignas(64) MapsI8 {
-    CUtensorMap q, w;
+    CUtensorMap q, w, y;
 };
 __device__ __forceinline__ void tc_mma_i8_lh(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -285,36 +301,33 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void store_32b(unsigned char* at, const uint32_t* w) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
-                 "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-// 64 bytes of each of a warp's rows to `y` (the first row's), `step` bytes from row to row: w = those of the lane's row; `have` bytes of
-// a row exist (a multiple of `size`, an element's bytes).  vec: bytes that may be stored at once everywhere in y.  Whole 64 bytes go
-// straight from the lanes where rows allow 16 bytes at once.  The rest passes through the warp's 32 x 64 bytes of shared memory, so
-// that the warp writes along the rows; the 16-byte pieces of a row lie in the pattern piece ^ (row / 2) % 4, free of bank conflicts.
-__device__ __forceinline__ void store_rows(const uint32_t* w, uint32_t* stage, unsigned char* y, long long step, int rows, int have, int vec, int size, int lane) {
-    if (vec >= 16 && have == 64) {
-        if (lane >= rows) return;
-        unsigned char* at = y + lane * step;
-        if (vec >= 32) {
-            store_32b(at, w);
-            store_32b(at + 32, w + 8);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(at + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        }
-        return;
-    }
+// 64 bytes of each of a warp's rows to y: w = those of the lane's row; they leave through the warp's 32 x 64 bytes of shared memory,
+// the 16-byte pieces of a row in the pattern piece ^ (row / 2) % 4 (the copy engine's 64-byte swizzle, free of bank conflicts).
+// Whole blocks go out as one tensor copy where y allows it (vec >= 16: bytes that may be stored at once everywhere in y; a copy that
+// ends inside 16 bytes of a row would write all of them).  A store by lanes, each 32 bytes of its own row, took 32 bytes a clock off the path that also feeds the tensor core: 65536 x
+// 1024 -> 2048 in 134 us against X.  The rest the warp writes along the rows.  x, row0: first byte of the row, first row; have: bytes
+// of a row that exist (a multiple of `size`, an element's bytes); step: bytes from row to row.
+__device__ __forceinline__ void store_rows(const uint32_t (&w)[16], uint32_t* stage, const void* tmap, unsigned char* base, int x, int row0, long long step, int rows,
+                                           int have, int vec, int size, int lane) {
     auto at = [&](int row, int word) { return stage + row * 16 + ((((word >> 2) ^ (row >> 1)) & 3) << 2) + (word & 3); };
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the copy before has read the buffer
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(at(lane, i)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    if (vec >= 16 && rows == 32 && have == 64) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(stage)), "r"(x), "r"(row0)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        return;
+    }
     __syncwarp();
     // half a warp a row
     const int col = lane & 15;
-    y += (lane >> 4) * step;
+    unsigned char* y = base + (long long)(row0 + (lane >> 4)) * step + x;
     for (int r0 = 0; r0 < rows; r0 += 2, y += 2 * step) {
         const int r = r0 + (lane >> 4);
         const uint32_t v = *at(r, col), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
@@ -392,13 +405,13 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *sA = smem, *sB = smem + NSTG * Cfg::A_STAGE;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + NSTG * Cfg::STAGE);
+    uint32_t* s_stage = reinterpret_cast<uint32_t*>(smem + NSTG * Cfg::STAGE);              // [epilogue warp][32][STAGED]
+    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][HN]: its channels' scales
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_ws + Cfg::EPI_WARPS * Cfg::HN);
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * NSTG, bar_tfull = bar_empty + 8 * NSTG, bar_tempty = bar_tfull + 8 * NBUF;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* s_stage = tmem_slot + 4;                                                      // [epilogue warp][32][STAGED]
-    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][HN]: its channels' scales
-    int2* s_range = reinterpret_cast<int2*>(s_ws + Cfg::EPI_WARPS * Cfg::HN);
+    int2* s_range = reinterpret_cast<int2*>(tmem_slot + 4);
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
@@ -595,7 +608,6 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
             if (t + units < tiles) fetch(t + units);
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * HN;
             const int n0 = now.n * BN + part * HN, size = p.dtype == TNNS_F32 ? 4 : 2;
-            unsigned char* y0 = (unsigned char*)p.y + ((long long)place0 * p.y_stride + n0) * size;
             const long long step = p.y_stride * size;
 #pragma unroll 1
             for (int i = 0; i < NC; i++) {
@@ -613,17 +625,18 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
                 const int have = (p.N - n0 - 32 * i) * size;
                 if (rows_here > 0 && have > 0) {
                     uint32_t w[16];
-                    unsigned char* y = y0 + 32 * i * size;
+                    const int x = (n0 + 32 * i) * size;
+                    unsigned char* base = reinterpret_cast<unsigned char*>(p.y);
                     if (size == 4) {
                         finish_words<16>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
-                        store_rows(w, stage, y, step, rows_here, min(have, 64), p.y_vec, 4, lane);
+                        store_rows(w, stage, &maps.y, base, x, place0, step, rows_here, min(have, 64), p.y_vec, 4, lane);
                         if (have > 64) {
                             finish_words<16>(p.dtype, v + 16, rs_now, wsc + 32 * i + 16, p.alpha, mode, w);
-                            store_rows(w, stage, y + 64, step, rows_here, min(have - 64, 64), p.y_vec, 4, lane);
+                            store_rows(w, stage, &maps.y, base, x + 64, place0, step, rows_here, min(have - 64, 64), p.y_vec, 4, lane);
                         }
                     } else {
                         finish_words<32>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
-                        store_rows(w, stage, y, step, rows_here, min(have, 64), p.y_vec, 2, lane);
+                        store_rows(w, stage, &maps.y, base, x, place0, step, rows_here, min(have, 64), p.y_vec, 2, lane);
                     }
                 }
                 __syncwarp();
@@ -633,6 +646,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
 
 done:
     __syncwarp();
+    if (warp >= Cfg::EPI0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // results still on their way out of shared memory
     if (*abort_flag && warp == WARP_TMA && lane == 0) {
         // a wait gave up: give the copies already requested time to land before shared memory is released
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
@@ -679,6 +693,11 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     if (rc) return rc;
     // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
     if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;
+    // y by bytes: boxes of 32 rows x 64 bytes
+    if (a.y_vec >= 16) {
+        const int size = tnns_dtype_bytes(a.dtype);
+        if ((rc = tnns_tensor_map_2d(&maps.y, 1, a.y, (unsigned long long)a.N * size, (unsigned long long)a.places, (unsigned long long)a.y_stride * size, 64, 32, 64))) return rc;
+    }
     auto kern = gemm_i8_tc_kernel<BN, CG, GATHER>;
     static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
     if (!smem_set[ctx->device & 63]) {
@@ -702,7 +721,7 @@ int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     const int wide = FEW_WARPS / S * 16;
     const long long items = high * ((a.N + wide - 1) / wide);
     if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
-    const int grid = (int)std::min<long long>(items, 8LL * ctx->sm_count);
+    const int grid = (int)std::min<long long>(items, 2LL * ctx->sm_count);  // as many blocks as are resident
     return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, S);
 }
 
@@ -725,7 +744,7 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     a.n_tiles = w->n_tiles; a.k_tiles = w->k_tiles; a.alpha = alpha;
     a.dtype = dtype; a.status = ctx->d_status;
     const uintptr_t at = (uintptr_t)d_y | (uintptr_t)(y_stride * tnns_dtype_bytes(dtype));
-    a.y_vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : at % 8 == 0 ? 8 : at % 4 == 0 ? 4 : 2;
+    a.y_vec = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
     const cudaStream_t st = (cudaStream_t)stream;
     // places an expert has on average
     const long long rows = (long long)places / w->experts;
@@ -745,7 +764,7 @@ int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float
                                 tnns_cuda_weights_i8** out) {
     if (!ctx || !w || !scales || !out) return tnns_fail(TNNS_ERR_INVALID, "NULL argument");
     *out = nullptr;
-    if (experts < 1 || experts > MAX_EXPERTS || N < 1 || K < 1 || K > 131071) return tnns_fail(TNNS_ERR_INVALID, "bad weight size: %d kernels (at most 1024) of %d x %d (K at most 131071)", experts, N, K);
+    if (experts < 1 || experts > MAX_EXPERTS || N < 1 || N > (1 << 28) || K < 1 || K > 131071) return tnns_fail(TNNS_ERR_INVALID, "bad weight size: %d kernels (at most 1024) of %d x %d (K at most 131071)", experts, N, K);
     int rc = tnns_enter(ctx);
     if (rc) return rc;
     tnns_cuda_weights_i8* h = new (std::nothrow) tnns_cuda_weights_i8();

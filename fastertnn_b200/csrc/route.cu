@@ -365,25 +365,31 @@ struct PlanArgs {
     int32_t* slots;
 };
 // Exclusive sums of s_v[0 .. n) by the whole block; s_v[n] = the total.
-__device__ __forceinline__ void scan_block(int* s_v, int n, int* s_part, int tid, int threads) {
+template <int THREADS>
+__device__ __forceinline__ void scan_block(int* s_v, int n, int* s_part, int tid) {
     const int lane = tid & 31, warp = tid >> 5;
     int carry = 0;
-    for (int b = 0; b < n; b += threads) {
+    for (int b = 0; b < n; b += THREADS) {
         const int v = b + tid < n ? s_v[b + tid] : 0;
         int x = v;
+#pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(FULL, x, d);
             if (lane >= d) x += o;
         }
         if (lane == 31) s_part[warp] = x;
         __syncthreads();
-        int before = carry;
-        for (int w = 0; w < warp; w++) before += s_part[w];
-        int total = carry;
-        for (int w = 0; w < (threads >> 5); w++) total += s_part[w];
-        if (b + tid < n) s_v[b + tid] = before + x - v;
-        carry = total;
-        __syncthreads();
+        // every warp sums the warps' parts for itself
+        int part = lane < THREADS / 32 ? s_part[lane] : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(FULL, part, d);
+            if (lane >= d) part += o;
+        }
+        const int before = warp ? __shfl_sync(FULL, part, warp - 1) : 0, total = __shfl_sync(FULL, part, 31);
+        if (b + tid < n) s_v[b + tid] = carry + before + x - v;
+        carry += total;
+        if (b + THREADS < n) __syncthreads();
     }
     if (tid == 0) s_v[n] = carry;
     __syncthreads();
@@ -477,7 +483,7 @@ __device__ __forceinline__ void plan_pairs(const RouteArgs& p, const PlanArgs& o
             for (int e = tid; e < E; e += THREADS) s_first[e] = s_count[e];
         }
         __syncthreads();
-        scan_block(s_first, E, s_part, tid, THREADS);
+        scan_block<THREADS>(s_first, E, s_part, tid);
         if (rank == 0)
             for (int e = tid; e <= E; e += THREADS) o.offsets[e] = s_first[e];
     }

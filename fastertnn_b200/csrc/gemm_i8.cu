@@ -115,6 +115,11 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void load_32b(const int8_t* at, uint4& lo, uint4& hi) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                 : "l"(at));
+}
 // 16 bytes of a row of q from byte k on; bytes behind K, which need not be readable, as zeros.
 __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
     if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
@@ -125,56 +130,84 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 
 // 8 * NT places x 16 channels a warp, or S warps that share the K tiles and add up their sums in shared memory; a block holds 8 / S
 // such pieces side by side and goes on to others, whose weights it requests before it finishes the present ones.  Bounded by the
-// weights' bytes: a lane (g, t) holds 16 bytes of pieces t and t + 4 of channels g and g + 8, so four instructions multiply a
-// whole K tile of 2 KB and no byte passes through shared memory.  The order of K within the tile is the same for weights and rows.
+// weights' bytes: a lane (g, t) holds the 32 bytes of pieces 2t and 2t + 1 of channels 2g and 2g + 1 (rows g and g + 8 of the
+// instruction), so a load takes eight whole lines, four instructions multiply a K tile of 2 KB, and no byte passes through shared
+// memory.  The order of K within the tile is the same for weights and rows.
 template <int NT>
-__global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int S) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int log_s) {
     constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
     extern __shared__ int2 s_range[];
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
+    __shared__ float s_scale[2][8 * NT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int ks = warp & (S - 1), wide = FEW_WARPS / S * 16, n_mine = (warp / S) * 16;  // this warp's part of K, channels of a block, the warp's among them
-    const int n_blocks = (p.N + wide - 1) / wide;
+    const int S = 1 << log_s, ks = warp & (S - 1), log_wide = 7 - log_s, wide = 1 << log_wide;  // this warp's part of K, channels of a block ..
+    const int n_mine = (warp >> log_s) * 16, n_out = tid & (wide - 1);                          // .. the first the warp multiplies, the one the thread finishes
+    const int n_blocks = (p.N + wide - 1) >> log_wide;
+    struct Item {
+        int e, m0, last, n0;  // expert, first place, end of the expert's places, first channel of the block
+    };
     const int8_t* wt = nullptr;
-    uint4 a[U][4];
+    uint4 a[U][4], x[U][NT][2];
+    int row[NT];     // of q, that the lane's places read; -1: none
+    float rs[NT], ws = 0.f;  // scales of those rows, of channel n_out
     auto load_weights = [&](int kt0) {
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (kt0 + u * S < p.k_tiles) {
                 const int8_t* tile = wt + (long long)(kt0 + u * S) * WT_BYTES;
-                a[u][0] = __ldg(reinterpret_cast<const uint4*>(tile + ((t ^ g) << 4)));
-                a[u][1] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + ((t ^ g) << 4)));
-                a[u][2] = __ldg(reinterpret_cast<const uint4*>(tile + (((t + 4) ^ g) << 4)));
-                a[u][3] = __ldg(reinterpret_cast<const uint4*>(tile + 1024 + (((t + 4) ^ g) << 4)));
+                load_32b(tile, a[u][0], a[u][1]);        // channel 2g: pieces 2t, 2t + 1
+                load_32b(tile + 128, a[u][3], a[u][2]);  // channel 2g + 1: the pattern has the two the other way round
             }
     };
-    // the warp's first weights of channels n .. of expert e
-    auto begin = [&](int e, int n) {
+    auto begin_weights = [&](int e, int n0) {
+        if (n0 + n_out < p.N) ws = __ldg(p.w_scale + (long long)e * p.n_tiles * WT + n0 + n_out);
+        const int n = n0 + n_mine;
         if (n >= p.N) return;
-        wt = p.img + ((long long)e * p.n_tiles + n / WT) * p.k_tiles * WT_BYTES + (n % WT + g) * 128;
+        wt = p.img + ((long long)e * p.n_tiles + n / WT) * p.k_tiles * WT_BYTES + (n % WT + 2 * g) * 128 + ((t ^ (g & 3)) << 5);
         load_weights(ks);
+    };
+    auto load_x = [&](int kt0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k0 = (kt0 + u * S) * WT;
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const int8_t* at = p.q + (long long)max(row[i], 0) * p.q_stride;
+                if (k0 + WT <= p.K) {  // a whole tile
+                    x[u][i][0] = row[i] >= 0 ? *reinterpret_cast<const uint4*>(at + k0 + t * 32) : make_uint4(0, 0, 0, 0);
+                    x[u][i][1] = row[i] >= 0 ? *reinterpret_cast<const uint4*>(at + k0 + t * 32 + 16) : make_uint4(0, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int k = k0 + t * 32 + h * 16;
+                        x[u][i][h] = row[i] >= 0 && k < p.K ? load_piece(at, k, p.K) : make_uint4(0, 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+    auto begin_rows = [&]() {
+        load_x(ks);
+#pragma unroll
+        for (int i = 0; i < NT; i++) rs[i] = row[i] >= 0 ? p.scale[row[i]] : 0.f;
     };
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // one kernel: the weights' way from memory starts before the launch in front has ended
-    if (!p.offsets) begin(0, (int)(blockIdx.x % (unsigned)n_blocks) * wide + n_mine);
+    if (!p.offsets) begin_weights(0, (int)(blockIdx.x % (unsigned)n_blocks) << log_wide);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     list_blocks<8 * NT>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, FEW_WARPS * 32);
     const int items = s_first[p.experts] * n_blocks;
-    struct Item {
-        int e, m0, last, n0;  // expert, first place, end of the expert's places, first channel of the block
-    };
     auto item_at = [&](int item) {
         Item r;
         const int b = item / n_blocks;
-        r.n0 = (item - b * n_blocks) * wide;
+        r.n0 = (item - b * n_blocks) << log_wide;
         r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
         const int2 range = s_range[r.e];
         r.m0 = range.x + (b - s_first[r.e]) * 8 * NT;
         r.last = range.y;
         return r;
     };
-    int row[NT];  // of q, that the lane's places read; -1: none
     auto rows_at = [&](const Item& c) {
 #pragma unroll
         for (int i = 0; i < NT; i++) {
@@ -186,61 +219,58 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __
     if ((int)blockIdx.x < items) {
         c = item_at(blockIdx.x);
         rows_at(c);
-        if (p.offsets) begin(c.e, c.n0 + n_mine);
+        if (p.offsets) begin_weights(c.e, c.n0);
+        begin_rows();
     }
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    for (int item = blockIdx.x, turn = 0; item < items; item += gridDim.x, turn ^= 1) {
+        const Item now = c;
+        const bool more = item + (int)gridDim.x < items;
         int acc[NT][4] = {};
-        if (c.n0 + n_mine < p.N) {
+        if (now.n0 + n_mine < p.N) {
             for (int kt0 = ks; kt0 < p.k_tiles; kt0 += S * U) {
-                uint4 x[U][NT][2];
-#pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int i = 0; i < NT; i++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int k = (kt0 + u * S) * WT + (t + 4 * h) * 16;
-                            x[u][i][h] = row[i] >= 0 && k < p.K ? load_piece(p.q + (long long)row[i] * p.q_stride, k, p.K) : make_uint4(0, 0, 0, 0);
-                        }
+                if (kt0 != ks) load_x(kt0);
 #pragma unroll
                 for (int u = 0; u < U; u++)
                     if (kt0 + u * S < p.k_tiles) {
 #pragma unroll
                         for (int i = 0; i < NT; i++) {
-                            mma_s8(acc[i], a[u][0].x, a[u][1].x, a[u][2].x, a[u][3].x, x[u][i][0].x, x[u][i][1].x);
-                            mma_s8(acc[i], a[u][0].y, a[u][1].y, a[u][2].y, a[u][3].y, x[u][i][0].y, x[u][i][1].y);
-                            mma_s8(acc[i], a[u][0].z, a[u][1].z, a[u][2].z, a[u][3].z, x[u][i][0].z, x[u][i][1].z);
-                            mma_s8(acc[i], a[u][0].w, a[u][1].w, a[u][2].w, a[u][3].w, x[u][i][0].w, x[u][i][1].w);
+                            mma_s8(acc[i], a[u][0].x, a[u][2].x, a[u][1].x, a[u][3].x, x[u][i][0].x, x[u][i][1].x);
+                            mma_s8(acc[i], a[u][0].y, a[u][2].y, a[u][1].y, a[u][3].y, x[u][i][0].y, x[u][i][1].y);
+                            mma_s8(acc[i], a[u][0].z, a[u][2].z, a[u][1].z, a[u][3].z, x[u][i][0].z, x[u][i][1].z);
+                            mma_s8(acc[i], a[u][0].w, a[u][2].w, a[u][1].w, a[u][3].w, x[u][i][0].w, x[u][i][1].w);
                         }
                     }
                 load_weights(kt0 + S * U);
             }
         }
-        const Item now = c;
-        if (item + (int)gridDim.x < items) {
-            c = item_at(item + gridDim.x);
-            rows_at(c);
-            begin(c.e, c.n0 + n_mine);
-        }
-        // d[0], d[1]: channel g, places 2t, 2t + 1; d[2], d[3]: channel g + 8
+        // d[0], d[1]: channel 2g, places 2t, 2t + 1; d[2], d[3]: channel 2g + 1
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) s_sum[warp][i][(2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = acc[i][j];
+            for (int j = 0; j < 4; j++) s_sum[warp][i][(2 * t + (j & 1)) * 16 + 2 * g + (j >> 1)] = acc[i][j];
+        if (warp == 0 && t == 0) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) s_scale[turn][i * 8 + g] = rs[i];
+        }
+        const float ws_now = ws;
+        if (more) {
+            c = item_at(item + gridDim.x);
+            rows_at(c);
+            begin_weights(c.e, c.n0);
+        }
         __syncthreads();
         // a result for each place and channel of the block, channels side by side
-        for (int o = tid; o < 8 * NT * wide; o += FEW_WARPS * 32) {
-            const int ch = o % wide, pl = o / wide, place = now.m0 + pl, n = now.n0 + ch;
-            if (place >= now.last || n >= p.N) continue;
-            int sum = 0;
-            for (int w = 0; w < S; w++) sum += s_sum[(ch >> 4) * S + w][pl >> 3][(pl & 7) * 16 + (ch & 15)];
-            const int r = row_of(p, place);
-            const float v = prelu((float)sum * (r >= 0 ? p.scale[r] : 0.f) * p.w_scale[(long long)now.e * p.n_tiles * WT + n], p.alpha);
-            const long long at = (long long)place * p.y_stride + n;
-            if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
-            else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
-            else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
-        }
+        if (now.n0 + n_out < p.N)
+            for (int pl = tid >> log_wide; pl < 8 * NT && now.m0 + pl < now.last; pl += FEW_WARPS * 32 >> log_wide) {
+                int sum = 0;
+                for (int w = 0; w < S; w++) sum += s_sum[((n_out >> 4) << log_s) + w][pl >> 3][(pl & 7) * 16 + (n_out & 15)];
+                const float v = prelu((float)sum * s_scale[turn][pl] * ws_now, p.alpha);
+                const long long at = (long long)(now.m0 + pl) * p.y_stride + now.n0 + n_out;
+                if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
+                else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
+                else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
+            }
+        if (more) begin_rows();
         __syncthreads();
     }
 }
@@ -716,13 +746,13 @@ template <int NT>
 int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     const long long high = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);  // at most
     const long long pieces = high * ((a.N + 15) / 16);
-    int S = 1;
-    while (S < FEW_WARPS && S < a.k_tiles && (a.k_tiles >= 8 * S || pieces * S < 2LL * FEW_WARPS * ctx->sm_count)) S *= 2;
-    const int wide = FEW_WARPS / S * 16;
+    int log_s = 0;
+    while (log_s < 3 && (1 << log_s) < a.k_tiles && (a.k_tiles >= 8 << log_s || pieces << log_s < 2LL * FEW_WARPS * ctx->sm_count)) log_s++;
+    const int wide = 128 >> log_s;
     const long long items = high * ((a.N + wide - 1) / wide);
     if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
     const int grid = (int)std::min<long long>(items, 2LL * ctx->sm_count);  // as many blocks as are resident
-    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, S);
+    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, log_s);
 }
 
 int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale, int q_rows,
@@ -747,12 +777,14 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     a.y_vec = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
     const cudaStream_t st = (cudaStream_t)stream;
     // places an expert has on average
-    const long long rows = (long long)places / w->experts;
+    const long long rows = ((long long)places + w->experts - 1) / w->experts;
     if (q_rows == 0 || rows <= 8) return launch_few<1>(ctx, a, st);
     if (rows <= 16) return launch_few<2>(ctx, a, st);
     const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
-    if (tiles >= ctx->sm_count / 2) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
-    if (tiles * 4 >= ctx->sm_count) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
+    // blocks of 128 rows: at least one for every expert that has a row
+    const long long high = std::max<long long>((places + 127) / 128, d_offsets ? std::min(w->experts, places) : 0);
+    if (tiles >= ctx->sm_count / 2 && rows > 128) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
+    if (high * ((w->N + 127) / 128) >= ctx->sm_count / 2) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
     return d_rows ? launch_tc<64, 1, true>(ctx, a, st) : launch_tc<64, 1, false>(ctx, a, st);
 }
 

@@ -363,6 +363,7 @@ struct PlanArgs {
     int32_t* offsets;
     int32_t* rows;
     int32_t* slots;
+    FastDiv by_k;  // pair -> token
 };
 // Exclusive sums of s_v[0 .. n) by the whole block; s_v[n] = the total.
 template <int THREADS>
@@ -410,54 +411,56 @@ __device__ __forceinline__ void plan_pairs(const RouteArgs& p, const PlanArgs& o
     const long long groups = ((long long)p.T + 31) / 32, each = (groups + RANKS - 1) / RANKS;
     const long long g0 = min(rank * each, groups), g1 = min(g0 + each, groups);
     const bool once = g1 - g0 <= high;
-    for (int e = tid; e < E; e += THREADS) s_count[e] = s_below[e] = 0;
+    for (int x = tid; x < E; x += THREADS) s_count[x] = s_below[x] = 0;
     __syncthreads();
-    auto place_of = [&](int i, int t0, int e) {  // pair i of expert e, of the slab that begins with token t0
-        const int t = (int)((unsigned)i / (unsigned)k) - t0;
-        return s_before[(t >> 5) * E + e] + __popc(s_mask[(t >> 5) * E + e] & ((1u << (t & 31)) - 1));
-    };
+    constexpr int U = 8;  // pairs of a thread whose loads are on their way together
+    int e[U];
     for (int pass = 0; pass < 2; pass++) {
         for (long long g = g0; g < g1; g += high) {
             const int here = (int)min((long long)high, g1 - g), t0 = (int)(g * 32), i0 = t0 * k, i1 = (int)min((long long)t0 + here * 32, (long long)p.T) * k;
+            const bool kept = once && i1 - i0 <= U * THREADS;  // pass 1 finds the experts in registers
+            auto load = [&](int i) {
+#pragma unroll
+                for (int u = 0; u < U; u++) e[u] = i + u * THREADS < i1 ? p.experts[i + u * THREADS] : -1;
+            };
             if (pass == 0 || !once) {
+                load(i0 + tid);
                 for (int i = tid; i < here * E; i += THREADS) s_mask[i] = 0;
                 __syncthreads();
-                for (int i = i0 + tid; i < i1; i += 4 * THREADS) {
-                    int e[4];
+                for (int i = i0 + tid; i < i1; i += U * THREADS) {
+                    if (i != i0 + tid) load(i);
 #pragma unroll
-                    for (int u = 0; u < 4; u++) e[u] = i + u * THREADS < i1 ? p.experts[i + u * THREADS] : -1;
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
+                    for (int u = 0; u < U; u++)
                         if (e[u] >= 0) {
-                            const int t = (int)((unsigned)(i + u * THREADS) / (unsigned)k) - t0;
+                            const int t = (int)o.by_k.div((uint32_t)(i + u * THREADS)) - t0;
                             atomicOr(&s_mask[(t >> 5) * E + e[u]], 1u << (t & 31));
                         }
                 }
                 __syncthreads();
-                for (int e = tid; e < E; e += THREADS) {
-                    int sum = pass == 0 ? s_count[e] : s_below[e];
+                int* s_run = pass == 0 ? s_count : s_below;
+                for (int x = tid; x < E; x += THREADS) {
+                    int sum = s_run[x];
 #pragma unroll 8
                     for (int h = 0; h < here; h++) {
-                        s_before[h * E + e] = sum;
-                        sum += __popc(s_mask[h * E + e]);
+                        s_before[h * E + x] = sum;
+                        sum += __popc(s_mask[h * E + x]);
                     }
-                    (pass == 0 ? s_count : s_below)[e] = sum;
+                    s_run[x] = sum;
                 }
                 __syncthreads();
             }
             if (pass == 1)
-                for (int i = i0 + tid; i < i1; i += 4 * THREADS) {
-                    int e[4];
+                for (int i = i0 + tid; i < i1; i += U * THREADS) {
+                    if (!kept) load(i);
 #pragma unroll
-                    for (int u = 0; u < 4; u++) e[u] = i + u * THREADS < i1 ? p.experts[i + u * THREADS] : -1;
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
+                    for (int u = 0; u < U; u++) {
                         const int j = i + u * THREADS;
                         if (j >= i1) break;
                         int at = -1;
                         if (e[u] >= 0) {
-                            at = s_first[e[u]] + (once ? s_below[e[u]] : 0) + place_of(j, t0, e[u]);
-                            o.rows[at] = (int)((unsigned)j / (unsigned)k);
+                            const int token = (int)o.by_k.div((uint32_t)j), t = token - t0, m = (t >> 5) * E + e[u];
+                            at = s_first[e[u]] + (once ? s_below[e[u]] : 0) + s_before[m] + __popc(s_mask[m] & ((1u << (t & 31)) - 1));
+                            o.rows[at] = token;
                         }
                         o.slots[j] = at;
                     }
@@ -639,7 +642,7 @@ int tnns_cuda_route(tnns_cuda_ctx* ctx, const tnns_route_t* r, const void* d_log
         return TNNS_OK;
     }
     PlanArgs o;
-    o.offsets = d_offsets; o.rows = d_rows; o.slots = d_slots;
+    o.offsets = d_offsets; o.rows = d_rows; o.slots = d_slots; o.by_k = tnns_fastdiv((uint32_t)r->top_k);
     TNNS_FOR_DTYPE(dtype, TI, return launch_route_npl<TI>(ctx, a, o, plan, st));
 }
 

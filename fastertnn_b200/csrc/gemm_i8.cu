@@ -66,6 +66,11 @@ __device__ __forceinline__ int row_of(const GemmI8Args& p, int place) {
 }
 __device__ __forceinline__ float prelu(float v, float alpha) { return v * (v > 0 ? 1.0f : alpha); }
 
+// All lanes of a warp wait; none leaves the loop before the others.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* status, unsigned code) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
+}
+
 // How a launch's work is dealt out: blocks of TM places of every expert, in the experts' order.  s_first[e] = blocks of the experts
 // before e, s_range[e] = the expert's places; called by the whole block, ends with a barrier.  Sums saturate at `limit` (overlapping
 // offsets are the caller's mistake), so that what is counted on from them stays an int.
@@ -276,6 +281,194 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __
 }
 
 // ---------------------------------------------------------------------------------------
+// Few rows for many experts: the same, fed by the copy engine
+// ---------------------------------------------------------------------------------------
+
+// A persistent block an SM takes pieces of 8 * NT places x 64 channels.  Their weights, 8 KB a K tile, come through a ring of bulk
+// copies that runs on across pieces, so that the bytes on their way do not wait for anything that happens to a piece.  Eight
+// warps: four times 16 channels, twice every other stage; the warps of a pair add their sums through shared memory and need no barrier
+// of the block.
+constexpr int RING_CH = 64, RING_STAGE = RING_CH * KCH, RING_SLOTS = 24, RING_FEW_THREADS = 32 * 9;
+static_assert(RING_SLOTS % 2 == 0, "a slot always belongs to the same four warps, whose waits on it are then successive phases");
+constexpr size_t ring_few_smem(int experts) { return 128 + (size_t)RING_SLOTS * RING_STAGE + list_bytes(experts); }
+template <int NT>
+__global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(const __grid_constant__ GemmI8Args p) {
+    constexpr int U = NT == 1 ? 4 : 2;  // stages of a warp whose rows' bytes are on their way together
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
+    int2* s_range = reinterpret_cast<int2*>(ring + RING_SLOTS * RING_STAGE);
+    int* s_first = reinterpret_cast<int*>(s_range + p.experts);
+    __shared__ uint64_t s_full[RING_SLOTS], s_empty[RING_SLOTS], s_sum_full[4], s_sum_empty[4];
+    __shared__ int s_sum[4][4 * NT][32];
+    __shared__ int s_abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t bar_full = smem_u32(s_full), bar_empty = smem_u32(s_empty), bar_sum_full = smem_u32(s_sum_full), bar_sum_empty = smem_u32(s_sum_empty);
+    if (tid == 0) {
+        for (int s = 0; s < RING_SLOTS; s++) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 4);
+        }
+        for (int s = 0; s < 4; s++) {
+            mbar_init(bar_sum_full + 8 * s, 1);
+            mbar_init(bar_sum_empty + 8 * s, 1);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int n_blocks = (p.N + RING_CH - 1) / RING_CH;
+    list_blocks<8 * NT>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, RING_FEW_THREADS);
+    const int items = s_first[p.experts] * n_blocks;
+    struct Item {
+        int e, m0, last, n0;  // expert, first place, end of the expert's places, first channel
+    };
+    auto item_at = [&](int item) {
+        Item r;
+        const int b = item / n_blocks;
+        r.n0 = (item - b * n_blocks) * RING_CH;
+        r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
+        const int2 range = s_range[r.e];
+        r.m0 = range.x + (b - s_first[r.e]) * 8 * NT;
+        r.last = range.y;
+        return r;
+    };
+    if (warp == 8) {
+        if (lane == 0) {
+            uint32_t s = 0, ph = 1;
+            for (int item = blockIdx.x; item < items; item += gridDim.x) {
+                const Item c = item_at(item);
+                const int8_t* src = p.img + ((long long)c.e * p.n_tiles + c.n0 / WT) * p.k_tiles * WT_BYTES + (c.n0 % WT) * KCH;
+                for (int kt = 0; kt < p.k_tiles; kt++, src += WT_BYTES) {
+                    if (!mbar_wait(bar_empty + 8 * s, ph, &s_abort, p.status, 14)) goto done;
+                    mbar_arrive_expect_tx(bar_full + 8 * s, RING_STAGE);
+                    bulk_g2s(smem_u32(ring + s * RING_STAGE), src, RING_STAGE, bar_full + 8 * s);
+                    if (++s == RING_SLOTS) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else {
+        const int group = warp & 1, cg = warp >> 1;  // stages of even or odd number; 16 channels
+        // bytes of the lane's pieces 2t and 2t + 1 of channels g and g + 8 within a slot (channel % 8 = g; free of bank conflicts)
+        const int lo = (cg * 16 + g) * KCH + (((2 * t) ^ g) << 4), hi = (cg * 16 + g) * KCH + (((2 * t + 1) ^ g) << 4);
+        uint32_t i0 = 0;  // number of the piece's first stage, modulo 2 * RING_SLOTS
+        uint32_t sums = 0;
+        for (int item = blockIdx.x; item < items; item += gridDim.x, i0 = (i0 + p.k_tiles) % (2 * RING_SLOTS), sums++) {
+            const Item c = item_at(item);
+            int row[NT];
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const int place = c.m0 + i * 8 + g;
+                row[i] = place < c.last ? row_of(p, place) : -1;
+            }
+            const int n = c.n0 + cg * 16 + g;  // and n + 8
+            float ws[2], rs[NT][2];
+            int acc[NT][4] = {};
+            uint4 x[2][U][NT][2];
+            auto load_x = [&](int kt0, uint4 (&d)[U][NT][2]) {  // of the warp's stages kt0, kt0 + 2, ..
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int k0 = (kt0 + 2 * u) * WT + t * 32;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const int8_t* at = p.q + (long long)max(row[i], 0) * p.q_stride;
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int k = k0 + 16 * h;
+                            d[u][i][h] = row[i] >= 0 && k < p.K ? load_piece(at, k, p.K) : make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                }
+            };
+            const int kt_first = ((int)i0 & 1) ^ group;  // the first K tile whose stage is the group's
+            load_x(kt_first, x[0]);
+            if (group == 0) {
+                const float* w = p.w_scale + (long long)c.e * p.n_tiles * WT;
+                ws[0] = n < p.N ? __ldg(w + n) : 0.f;
+                ws[1] = n + 8 < p.N ? __ldg(w + n + 8) : 0.f;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int place = c.m0 + i * 8 + 2 * t + j, r = place < c.last ? row_of(p, place) : -1;
+                        rs[i][j] = r >= 0 ? p.scale[r] : 0.f;
+                    }
+            }
+            int turn = 0;
+            for (int kt0 = kt_first; kt0 < p.k_tiles; kt0 += 4 * U) {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int kb = kt0 + 2 * U * b;
+                    if (kb < p.k_tiles) {
+                        if (kb + 2 * U < p.k_tiles) load_x(kb + 2 * U, x[b ^ 1]);
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            const int kt = kb + 2 * u;
+                            if (kt < p.k_tiles) {
+                                const uint32_t at = (i0 + (uint32_t)kt) % (2 * RING_SLOTS), s = at % RING_SLOTS;
+                                if (!warp_wait(bar_full + 8 * s, at < RING_SLOTS ? 0u : 1u, &s_abort, p.status, 15)) goto done;
+                                const unsigned char* slot = ring + s * RING_STAGE;
+                                const uint4 a0 = *reinterpret_cast<const uint4*>(slot + lo), a1 = *reinterpret_cast<const uint4*>(slot + lo + 8 * KCH);
+                                const uint4 a2 = *reinterpret_cast<const uint4*>(slot + hi), a3 = *reinterpret_cast<const uint4*>(slot + hi + 8 * KCH);
+#pragma unroll
+                                for (int i = 0; i < NT; i++) {
+                                    mma_s8(acc[i], a0.x, a1.x, a2.x, a3.x, x[b][u][i][0].x, x[b][u][i][1].x);
+                                    mma_s8(acc[i], a0.y, a1.y, a2.y, a3.y, x[b][u][i][0].y, x[b][u][i][1].y);
+                                    mma_s8(acc[i], a0.z, a1.z, a2.z, a3.z, x[b][u][i][0].z, x[b][u][i][1].z);
+                                    mma_s8(acc[i], a0.w, a1.w, a2.w, a3.w, x[b][u][i][0].w, x[b][u][i][1].w);
+                                }
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+                            }
+                        }
+                    }
+                }
+            }
+            // the second warp of a pair hands its sums to the first
+            if (group == 1) {
+                if (!warp_wait(bar_sum_empty + 8 * cg, (sums & 1) ^ 1, &s_abort, p.status, 16)) goto done;
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s_sum[cg][4 * i + j][lane] = acc[i][j];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_sum_full + 8 * cg);
+                continue;
+            }
+            if (!warp_wait(bar_sum_full + 8 * cg, sums & 1, &s_abort, p.status, 17)) goto done;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] += s_sum[cg][4 * i + j][lane];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_sum_empty + 8 * cg);
+            // acc[0], [1]: channel n, places 2t, 2t + 1; [2], [3]: channel n + 8
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int place = c.m0 + i * 8 + 2 * t + (j & 1), ch = n + 8 * (j >> 1);
+                    if (place < c.last && ch < p.N) {
+                        const float v = prelu((float)acc[i][j] * rs[i][j & 1] * ws[j >> 1], p.alpha);
+                        const long long at = (long long)place * p.y_stride + ch;
+                        if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
+                        else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
+                        else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
+                    }
+                }
+        }
+    }
+done:
+    __syncwarp();
+    if (s_abort && warp == 8 && lane == 0) {
+        // a wait gave up: give the copies already requested time to land before shared memory is released
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------
 // Many rows: 5th-generation tensor cores, accumulators in tensor memory
 // ---------------------------------------------------------------------------------------
 
@@ -414,11 +607,6 @@ __device__ __forceinline__ void finish_words(int dtype, const uint32_t* v, float
             w[j / 2 + 1] = *reinterpret_cast<const uint32_t*>(&y);
         }
     }
-}
-
-// All lanes of a warp wait; none leaves the loop before the others.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* status, unsigned code) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
 }
 
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
@@ -741,6 +929,20 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
 }
 
+template <int NT>
+int launch_few_ring(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
+    auto kern = gemm_i8_few_ring_kernel<NT>;
+    static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
+    if (!smem_set[ctx->device & 63]) {
+        TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_few_smem(MAX_EXPERTS)));
+        smem_set[ctx->device & 63] = true;
+    }
+    const long long high = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);  // at most
+    const long long items = high * ((a.N + RING_CH - 1) / RING_CH);
+    if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
+    return launch<GemmI8Args>(kern, ctx, (int)std::min<long long>(items, ctx->sm_count), RING_FEW_THREADS, ring_few_smem(a.experts), 1, stream, a);
+}
+
 // Warps that share the K tiles: at least four tiles a warp, so that their loads overlap, unless the pieces do not fill the SMs.
 template <int NT>
 int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
@@ -778,8 +980,11 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const cudaStream_t st = (cudaStream_t)stream;
     // places an expert has on average
     const long long rows = ((long long)places + w->experts - 1) / w->experts;
-    if (q_rows == 0 || rows <= 8) return launch_few<1>(ctx, a, st);
-    if (rows <= 16) return launch_few<2>(ctx, a, st);
+    // pieces of the ring form: a block for every expert that has a row
+    const long long pieces = (long long)std::min(w->experts, places) * ((w->N + RING_CH - 1) / RING_CH);
+    const bool ring = d_offsets && pieces >= ctx->sm_count;
+    if (q_rows == 0 || rows <= 8) return ring ? launch_few_ring<1>(ctx, a, st) : launch_few<1>(ctx, a, st);
+    if (rows <= 16) return ring ? launch_few_ring<2>(ctx, a, st) : launch_few<2>(ctx, a, st);
     const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
     // blocks of 128 rows: at least one for every expert that has a row
     const long long high = std::max<long long>((places + 127) / 128, d_offsets ? std::min(w->experts, places) : 0);

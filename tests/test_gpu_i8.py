@@ -311,7 +311,8 @@ COUNTS = [
     ([128, 129, 127, 1], 384, 256), ([300, 0, 12, 500], 640, 520), ([5] * 150, 96, 130), ([1000, 3, 1, 700], 1024, 264), ([2] * 300 + [0] * 20, 64, 70),
     ([2000], 256, 513), ([40] * 30, 1100, 257), ([16] * 20 + [1], 777, 1000), ([3000, 2500], 500, 1300),
     ([700, 1, 900, 0, 257, 256, 255, 1400], 640, 2100),
-    ([130] * 60, 2048, 1024), ([60] * 40, 4000, 200), ([90] * 6, 6000, 300)]
+    ([130] * 60, 2048, 1024), ([60] * 40, 4000, 200), ([90] * 6, 6000, 300),
+    ([3, 0, 9, 1] * 20, 2000, 700), ([12, 20] * 30, 1300, 384), ([1] * 200, 130, 65), ([7] * 40, 5003, 1024)]
 
 
 @pytest.mark.parametrize("gather", [True, False])

@@ -285,21 +285,21 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __
 // ---------------------------------------------------------------------------------------
 
 // A persistent block an SM takes pieces of 8 * NT places x 64 channels.  Their weights, 8 KB a K tile, come through a ring of bulk
-// copies that runs on across pieces, so that the bytes on their way do not wait for anything that happens to a piece.  Eight
-// warps: four times 16 channels, twice every other stage; the warps of a pair add their sums through shared memory and need no barrier
-// of the block.
-constexpr int RING_CH = 64, RING_STAGE = RING_CH * KCH, RING_SLOTS = 24, RING_FEW_THREADS = 32 * 9;
-static_assert(RING_SLOTS % 2 == 0, "a slot always belongs to the same four warps, whose waits on it are then successive phases");
+// copies that runs on across pieces, so that the bytes on their way do not wait for anything that happens to a piece.  Sixteen
+// warps: four times 16 channels, four times every fourth stage; a warp asks for the rows' bytes of its next stage, and of the next piece,
+// ahead.  The four warps of the same channels add their sums through shared memory and need no barrier of the block.  (With eight warps
+// and each stage's position worked out anew, the warps' instructions were the bound: 25 against X us.)
+constexpr int RING_CH = 64, RING_STAGE = RING_CH * KCH, RING_SLOTS = 24, RING_GROUPS = 4, RING_FEW_THREADS = 32 * (4 * RING_GROUPS + 1);
+static_assert(RING_SLOTS % RING_GROUPS == 0, "a slot always belongs to the same four warps, whose waits on it are then successive phases");
 constexpr size_t ring_few_smem(int experts) { return 128 + (size_t)RING_SLOTS * RING_STAGE + list_bytes(experts); }
 template <int NT>
 __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(const __grid_constant__ GemmI8Args p) {
-    constexpr int U = NT == 1 ? 4 : 2;  // stages of a warp whose rows' bytes are on their way together
     extern __shared__ unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
     int2* s_range = reinterpret_cast<int2*>(ring + RING_SLOTS * RING_STAGE);
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     __shared__ uint64_t s_full[RING_SLOTS], s_empty[RING_SLOTS], s_sum_full[4], s_sum_empty[4];
-    __shared__ int s_sum[4][4 * NT][32];
+    __shared__ int s_sum[4][RING_GROUPS - 1][4 * NT][32];
     __shared__ int s_abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t bar_full = smem_u32(s_full), bar_empty = smem_u32(s_empty), bar_sum_full = smem_u32(s_sum_full), bar_sum_empty = smem_u32(s_sum_empty);
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
             mbar_init(bar_empty + 8 * s, 4);
         }
         for (int s = 0; s < 4; s++) {
-            mbar_init(bar_sum_full + 8 * s, 1);
+            mbar_init(bar_sum_full + 8 * s, RING_GROUPS - 1);
             mbar_init(bar_sum_empty + 8 * s, 1);
         }
         s_abort = 0;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
         r.last = range.y;
         return r;
     };
-    if (warp == 8) {
+    if (warp == 4 * RING_GROUPS) {
         if (lane == 0) {
             uint32_t s = 0, ph = 1;
             for (int item = blockIdx.x; item < items; item += gridDim.x) {
@@ -349,89 +349,118 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
             }
         }
     } else {
-        const int group = warp & 1, cg = warp >> 1;  // stages of even or odd number; 16 channels
+        const int group = warp / 4, cg = warp & 3;  // stages of number group modulo RING_GROUPS; 16 channels
         // bytes of the lane's pieces 2t and 2t + 1 of channels g and g + 8 within a slot (channel % 8 = g; free of bank conflicts)
-        const int lo = (cg * 16 + g) * KCH + (((2 * t) ^ g) << 4), hi = (cg * 16 + g) * KCH + (((2 * t + 1) ^ g) << 4);
-        uint32_t i0 = 0;  // number of the piece's first stage, modulo 2 * RING_SLOTS
+        const unsigned char* lo = ring + (cg * 16 + g) * KCH + (((2 * t) ^ g) << 4);
+        const int to_hi = ((((2 * t + 1) ^ g) - ((2 * t) ^ g)) << 4);
+        uint32_t s = group, ph = 0;  // the warp's next slot, and the parity its "full" barrier is waited with
+        int kt = group;              // the piece's first K tile whose stage is the group's
         uint32_t sums = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x, i0 = (i0 + p.k_tiles) % (2 * RING_SLOTS), sums++) {
-            const Item c = item_at(item);
-            int row[NT];
+        int row[NT];
+        uint4 x[NT][2];
+        auto rows_at = [&](const Item& c) {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
                 const int place = c.m0 + i * 8 + g;
                 row[i] = place < c.last ? row_of(p, place) : -1;
             }
-            const int n = c.n0 + cg * 16 + g;  // and n + 8
-            float ws[2], rs[NT][2];
-            int acc[NT][4] = {};
-            uint4 x[2][U][NT][2];
-            auto load_x = [&](int kt0, uint4 (&d)[U][NT][2]) {  // of the warp's stages kt0, kt0 + 2, ..
+        };
+        // the rows' bytes of K tile k; lanes without a row keep the zeros that they hold
+        auto load_x = [&](int k, uint4 (&d)[NT][2]) {
+            if (k >= p.k_tiles) return;
+            const int k0 = k * WT + t * 32;
+            if ((k + 1) * WT <= p.K) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int k0 = (kt0 + 2 * u) * WT + t * 32;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        const int8_t* at = p.q + (long long)max(row[i], 0) * p.q_stride;
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int k = k0 + 16 * h;
-                            d[u][i][h] = row[i] >= 0 && k < p.K ? load_piece(at, k, p.K) : make_uint4(0, 0, 0, 0);
-                        }
+                for (int i = 0; i < NT; i++)
+                    if (row[i] >= 0) {
+                        const uint4* at = reinterpret_cast<const uint4*>(p.q + (long long)row[i] * p.q_stride + k0);
+                        d[i][0] = at[0];
+                        d[i][1] = at[1];
                     }
-                }
-            };
-            const int kt_first = ((int)i0 & 1) ^ group;  // the first K tile whose stage is the group's
-            load_x(kt_first, x[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        d[i][h] = row[i] >= 0 && k0 + 16 * h < p.K ? load_piece(p.q + (long long)row[i] * p.q_stride, k0 + 16 * h, p.K) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto clear = [&](uint4 (&d)[NT][2]) {
+#pragma unroll
+            for (int i = 0; i < NT; i++) d[i][0] = d[i][1] = make_uint4(0, 0, 0, 0);
+        };
+        Item c = {};
+        if ((int)blockIdx.x < items) {
+            c = item_at(blockIdx.x);
+            rows_at(c);
+            clear(x);
+            load_x(kt, x);
+        }
+        for (int item = blockIdx.x; item < items; item += gridDim.x, sums++) {
+            const Item now = c;
+            const int n = now.n0 + cg * 16 + g;  // and n + 8
+            float ws[2] = {0.f, 0.f}, rs[NT][2];
             if (group == 0) {
-                const float* w = p.w_scale + (long long)c.e * p.n_tiles * WT;
-                ws[0] = n < p.N ? __ldg(w + n) : 0.f;
-                ws[1] = n + 8 < p.N ? __ldg(w + n + 8) : 0.f;
+                const float* w = p.w_scale + (long long)now.e * p.n_tiles * WT;
+                if (n < p.N) ws[0] = __ldg(w + n);
+                if (n + 8 < p.N) ws[1] = __ldg(w + n + 8);
 #pragma unroll
                 for (int i = 0; i < NT; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const int place = c.m0 + i * 8 + 2 * t + j, r = place < c.last ? row_of(p, place) : -1;
+                        const int place = now.m0 + i * 8 + 2 * t + j, r = place < now.last ? row_of(p, place) : -1;
                         rs[i][j] = r >= 0 ? p.scale[r] : 0.f;
                     }
             }
-            int turn = 0;
-            for (int kt0 = kt_first; kt0 < p.k_tiles; kt0 += 4 * U) {
+            const bool more = item + (int)gridDim.x < items;
+            int row_next[NT];
+            if (more) {
+                c = item_at(item + gridDim.x);
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const int kb = kt0 + 2 * U * b;
-                    if (kb < p.k_tiles) {
-                        if (kb + 2 * U < p.k_tiles) load_x(kb + 2 * U, x[b ^ 1]);
-#pragma unroll
-                        for (int u = 0; u < U; u++) {
-                            const int kt = kb + 2 * u;
-                            if (kt < p.k_tiles) {
-                                const uint32_t at = (i0 + (uint32_t)kt) % (2 * RING_SLOTS), s = at % RING_SLOTS;
-                                if (!warp_wait(bar_full + 8 * s, at < RING_SLOTS ? 0u : 1u, &s_abort, p.status, 15)) goto done;
-                                const unsigned char* slot = ring + s * RING_STAGE;
-                                const uint4 a0 = *reinterpret_cast<const uint4*>(slot + lo), a1 = *reinterpret_cast<const uint4*>(slot + lo + 8 * KCH);
-                                const uint4 a2 = *reinterpret_cast<const uint4*>(slot + hi), a3 = *reinterpret_cast<const uint4*>(slot + hi + 8 * KCH);
-#pragma unroll
-                                for (int i = 0; i < NT; i++) {
-                                    mma_s8(acc[i], a0.x, a1.x, a2.x, a3.x, x[b][u][i][0].x, x[b][u][i][1].x);
-                                    mma_s8(acc[i], a0.y, a1.y, a2.y, a3.y, x[b][u][i][0].y, x[b][u][i][1].y);
-                                    mma_s8(acc[i], a0.z, a1.z, a2.z, a3.z, x[b][u][i][0].z, x[b][u][i][1].z);
-                                    mma_s8(acc[i], a0.w, a1.w, a2.w, a3.w, x[b][u][i][0].w, x[b][u][i][1].w);
-                                }
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(bar_empty + 8 * s);
-                            }
-                        }
-                    }
+                for (int i = 0; i < NT; i++) {
+                    const int place = c.m0 + i * 8 + g;
+                    row_next[i] = place < c.last ? row_of(p, place) : -1;
                 }
             }
-            // the second warp of a pair hands its sums to the first
-            if (group == 1) {
+            int acc[NT][4] = {};
+            for (; kt < p.k_tiles; kt += RING_GROUPS) {
+                uint4 ahead[NT][2];
+                clear(ahead);
+                load_x(kt + RING_GROUPS, ahead);
+                if (!warp_wait(bar_full + 8 * s, ph, &s_abort, p.status, 15)) goto done;
+                const unsigned char* slot = lo + s * RING_STAGE;
+                const uint4 a0 = *reinterpret_cast<const uint4*>(slot), a1 = *reinterpret_cast<const uint4*>(slot + 8 * KCH);
+                const uint4 a2 = *reinterpret_cast<const uint4*>(slot + to_hi), a3 = *reinterpret_cast<const uint4*>(slot + to_hi + 8 * KCH);
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    mma_s8(acc[i], a0.x, a1.x, a2.x, a3.x, x[i][0].x, x[i][1].x);
+                    mma_s8(acc[i], a0.y, a1.y, a2.y, a3.y, x[i][0].y, x[i][1].y);
+                    mma_s8(acc[i], a0.z, a1.z, a2.z, a3.z, x[i][0].z, x[i][1].z);
+                    mma_s8(acc[i], a0.w, a1.w, a2.w, a3.w, x[i][0].w, x[i][1].w);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+                if ((s += RING_GROUPS) >= RING_SLOTS) { s -= RING_SLOTS; ph ^= 1; }
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    x[i][0] = ahead[i][0];
+                    x[i][1] = ahead[i][1];
+                }
+            }
+            kt -= p.k_tiles;  // stages are numbered on across pieces
+            if (more) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) row[i] = row_next[i];
+                clear(x);
+                load_x(kt, x);
+            }
+            // the warps of the same channels hand their sums to the first
+            if (group != 0) {
                 if (!warp_wait(bar_sum_empty + 8 * cg, (sums & 1) ^ 1, &s_abort, p.status, 16)) goto done;
 #pragma unroll
                 for (int i = 0; i < NT; i++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s_sum[cg][4 * i + j][lane] = acc[i][j];
+                    for (int j = 0; j < 4; j++) s_sum[cg][group - 1][4 * i + j][lane] = acc[i][j];
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_sum_full + 8 * cg);
                 continue;
@@ -440,7 +469,9 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] += s_sum[cg][4 * i + j][lane];
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int o = 0; o < RING_GROUPS - 1; o++) acc[i][j] += s_sum[cg][o][4 * i + j][lane];
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_sum_empty + 8 * cg);
             // acc[0], [1]: channel n, places 2t, 2t + 1; [2], [3]: channel n + 8
@@ -448,8 +479,8 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
             for (int i = 0; i < NT; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int place = c.m0 + i * 8 + 2 * t + (j & 1), ch = n + 8 * (j >> 1);
-                    if (place < c.last && ch < p.N) {
+                    const int place = now.m0 + i * 8 + 2 * t + (j & 1), ch = n + 8 * (j >> 1);
+                    if (place < now.last && ch < p.N) {
                         const float v = prelu((float)acc[i][j] * rs[i][j & 1] * ws[j >> 1], p.alpha);
                         const long long at = (long long)place * p.y_stride + ch;
                         if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
@@ -461,7 +492,7 @@ __global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(c
     }
 done:
     __syncwarp();
-    if (s_abort && warp == 8 && lane == 0) {
+    if (s_abort && warp == 4 * RING_GROUPS && lane == 0) {
         // a wait gave up: give the copies already requested time to land before shared memory is released
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }

@@ -49,6 +49,7 @@ struct GemmI8Args {
     long long y_stride;
     int q_rows, places, experts, N, K, n_tiles, k_tiles;
     int dtype, y_vec;  // result type; bytes that may be stored at once everywhere in y
+    int q_box;         // rows of a tensor copy of q
     float alpha;
     unsigned int* status;
 };
@@ -281,225 +282,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows for many experts: the same, fed by the copy engine
-// ---------------------------------------------------------------------------------------
-
-// A persistent block an SM takes pieces of 8 * NT places x 64 channels.  Their weights, 8 KB a K tile, come through a ring of bulk
-// copies that runs on across pieces, so that the bytes on their way do not wait for anything that happens to a piece.  Sixteen
-// warps: four times 16 channels, four times every fourth stage; a warp asks for the rows' bytes of its next stage, and of the next piece,
-// ahead.  The four warps of the same channels add their sums through shared memory and need no barrier of the block.  (With eight warps
-// and each stage's position worked out anew, the warps' instructions were the bound: 25 against X us.)
-constexpr int RING_CH = 64, RING_STAGE = RING_CH * KCH, RING_SLOTS = 24, RING_GROUPS = 4, RING_FEW_THREADS = 32 * (4 * RING_GROUPS + 1);
-static_assert(RING_SLOTS % RING_GROUPS == 0, "a slot always belongs to the same four warps, whose waits on it are then successive phases");
-constexpr size_t ring_few_smem(int experts) { return 128 + (size_t)RING_SLOTS * RING_STAGE + list_bytes(experts); }
-template <int NT>
-__global__ void __launch_bounds__(RING_FEW_THREADS, 1) gemm_i8_few_ring_kernel(const __grid_constant__ GemmI8Args p) {
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~(uintptr_t)127);
-    int2* s_range = reinterpret_cast<int2*>(ring + RING_SLOTS * RING_STAGE);
-    int* s_first = reinterpret_cast<int*>(s_range + p.experts);
-    __shared__ uint64_t s_full[RING_SLOTS], s_empty[RING_SLOTS], s_sum_full[4], s_sum_empty[4];
-    __shared__ int s_sum[4][RING_GROUPS - 1][4 * NT][32];
-    __shared__ int s_abort;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t bar_full = smem_u32(s_full), bar_empty = smem_u32(s_empty), bar_sum_full = smem_u32(s_sum_full), bar_sum_empty = smem_u32(s_sum_empty);
-    if (tid == 0) {
-        for (int s = 0; s < RING_SLOTS; s++) {
-            mbar_init(bar_full + 8 * s, 1);
-            mbar_init(bar_empty + 8 * s, 4);
-        }
-        for (int s = 0; s < 4; s++) {
-            mbar_init(bar_sum_full + 8 * s, RING_GROUPS - 1);
-            mbar_init(bar_sum_empty + 8 * s, 1);
-        }
-        s_abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncthreads();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int n_blocks = (p.N + RING_CH - 1) / RING_CH;
-    list_blocks<8 * NT>(p, s_range, s_first, 0x7FFFFFFFu / n_blocks / 2, tid, RING_FEW_THREADS);
-    const int items = s_first[p.experts] * n_blocks;
-    struct Item {
-        int e, m0, last, n0;  // expert, first place, end of the expert's places, first channel
-    };
-    auto item_at = [&](int item) {
-        Item r;
-        const int b = item / n_blocks;
-        r.n0 = (item - b * n_blocks) * RING_CH;
-        r.e = p.experts == 1 ? 0 : expert_of(s_first, p.experts, b);
-        const int2 range = s_range[r.e];
-        r.m0 = range.x + (b - s_first[r.e]) * 8 * NT;
-        r.last = range.y;
-        return r;
-    };
-    if (warp == 4 * RING_GROUPS) {
-        if (lane == 0) {
-            uint32_t s = 0, ph = 1;
-            for (int item = blockIdx.x; item < items; item += gridDim.x) {
-                const Item c = item_at(item);
-                const int8_t* src = p.img + ((long long)c.e * p.n_tiles + c.n0 / WT) * p.k_tiles * WT_BYTES + (c.n0 % WT) * KCH;
-                for (int kt = 0; kt < p.k_tiles; kt++, src += WT_BYTES) {
-                    if (!mbar_wait(bar_empty + 8 * s, ph, &s_abort, p.status, 14)) goto done;
-                    mbar_arrive_expect_tx(bar_full + 8 * s, RING_STAGE);
-                    bulk_g2s(smem_u32(ring + s * RING_STAGE), src, RING_STAGE, bar_full + 8 * s);
-                    if (++s == RING_SLOTS) { s = 0; ph ^= 1; }
-                }
-            }
-        }
-    } else {
-        const int group = warp / 4, cg = warp & 3;  // stages of number group modulo RING_GROUPS; 16 channels
-        // bytes of the lane's pieces 2t and 2t + 1 of channels g and g + 8 within a slot (channel % 8 = g; free of bank conflicts)
-        const unsigned char* lo = ring + (cg * 16 + g) * KCH + (((2 * t) ^ g) << 4);
-        const int to_hi = ((((2 * t + 1) ^ g) - ((2 * t) ^ g)) << 4);
-        uint32_t s = group, ph = 0;  // the warp's next slot, and the parity its "full" barrier is waited with
-        int kt = group;              // the piece's first K tile whose stage is the group's
-        uint32_t sums = 0;
-        int row[NT];
-        uint4 x[NT][2];
-        auto rows_at = [&](const Item& c) {
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const int place = c.m0 + i * 8 + g;
-                row[i] = place < c.last ? row_of(p, place) : -1;
-            }
-        };
-        // the rows' bytes of K tile k; lanes without a row keep the zeros that they hold
-        auto load_x = [&](int k, uint4 (&d)[NT][2]) {
-            if (k >= p.k_tiles) return;
-            const int k0 = k * WT + t * 32;
-            if ((k + 1) * WT <= p.K) {
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-                    if (row[i] >= 0) {
-                        const uint4* at = reinterpret_cast<const uint4*>(p.q + (long long)row[i] * p.q_stride + k0);
-                        d[i][0] = at[0];
-                        d[i][1] = at[1];
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        d[i][h] = row[i] >= 0 && k0 + 16 * h < p.K ? load_piece(p.q + (long long)row[i] * p.q_stride, k0 + 16 * h, p.K) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto clear = [&](uint4 (&d)[NT][2]) {
-#pragma unroll
-            for (int i = 0; i < NT; i++) d[i][0] = d[i][1] = make_uint4(0, 0, 0, 0);
-        };
-        Item c = {};
-        if ((int)blockIdx.x < items) {
-            c = item_at(blockIdx.x);
-            rows_at(c);
-            clear(x);
-            load_x(kt, x);
-        }
-        for (int item = blockIdx.x; item < items; item += gridDim.x, sums++) {
-            const Item now = c;
-            const int n = now.n0 + cg * 16 + g;  // and n + 8
-            float ws[2] = {0.f, 0.f}, rs[NT][2];
-            if (group == 0) {
-                const float* w = p.w_scale + (long long)now.e * p.n_tiles * WT;
-                if (n < p.N) ws[0] = __ldg(w + n);
-                if (n + 8 < p.N) ws[1] = __ldg(w + n + 8);
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int place = now.m0 + i * 8 + 2 * t + j, r = place < now.last ? row_of(p, place) : -1;
-                        rs[i][j] = r >= 0 ? p.scale[r] : 0.f;
-                    }
-            }
-            const bool more = item + (int)gridDim.x < items;
-            int row_next[NT];
-            if (more) {
-                c = item_at(item + gridDim.x);
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const int place = c.m0 + i * 8 + g;
-                    row_next[i] = place < c.last ? row_of(p, place) : -1;
-                }
-            }
-            int acc[NT][4] = {};
-            for (; kt < p.k_tiles; kt += RING_GROUPS) {
-                uint4 ahead[NT][2];
-                clear(ahead);
-                load_x(kt + RING_GROUPS, ahead);
-                if (!warp_wait(bar_full + 8 * s, ph, &s_abort, p.status, 15)) goto done;
-                const unsigned char* slot = lo + s * RING_STAGE;
-                const uint4 a0 = *reinterpret_cast<const uint4*>(slot), a1 = *reinterpret_cast<const uint4*>(slot + 8 * KCH);
-                const uint4 a2 = *reinterpret_cast<const uint4*>(slot + to_hi), a3 = *reinterpret_cast<const uint4*>(slot + to_hi + 8 * KCH);
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    mma_s8(acc[i], a0.x, a1.x, a2.x, a3.x, x[i][0].x, x[i][1].x);
-                    mma_s8(acc[i], a0.y, a1.y, a2.y, a3.y, x[i][0].y, x[i][1].y);
-                    mma_s8(acc[i], a0.z, a1.z, a2.z, a3.z, x[i][0].z, x[i][1].z);
-                    mma_s8(acc[i], a0.w, a1.w, a2.w, a3.w, x[i][0].w, x[i][1].w);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_empty + 8 * s);
-                if ((s += RING_GROUPS) >= RING_SLOTS) { s -= RING_SLOTS; ph ^= 1; }
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    x[i][0] = ahead[i][0];
-                    x[i][1] = ahead[i][1];
-                }
-            }
-            kt -= p.k_tiles;  // stages are numbered on across pieces
-            if (more) {
-#pragma unroll
-                for (int i = 0; i < NT; i++) row[i] = row_next[i];
-                clear(x);
-                load_x(kt, x);
-            }
-            // the warps of the same channels hand their sums to the first
-            if (group != 0) {
-                if (!warp_wait(bar_sum_empty + 8 * cg, (sums & 1) ^ 1, &s_abort, p.status, 16)) goto done;
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s_sum[cg][group - 1][4 * i + j][lane] = acc[i][j];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_sum_full + 8 * cg);
-                continue;
-            }
-            if (!warp_wait(bar_sum_full + 8 * cg, sums & 1, &s_abort, p.status, 17)) goto done;
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int o = 0; o < RING_GROUPS - 1; o++) acc[i][j] += s_sum[cg][o][4 * i + j][lane];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_sum_empty + 8 * cg);
-            // acc[0], [1]: channel n, places 2t, 2t + 1; [2], [3]: channel n + 8
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int place = now.m0 + i * 8 + 2 * t + (j & 1), ch = n + 8 * (j >> 1);
-                    if (place < now.last && ch < p.N) {
-                        const float v = prelu((float)acc[i][j] * rs[i][j & 1] * ws[j >> 1], p.alpha);
-                        const long long at = (long long)place * p.y_stride + ch;
-                        if (p.dtype == TNNS_F32) ((float*)p.y)[at] = v;
-                        else if (p.dtype == TNNS_F16) ((__half*)p.y)[at] = __float2half_rn(v);
-                        else ((__nv_bfloat16*)p.y)[at] = __float2bfloat16_rn(v);
-                    }
-                }
-        }
-    }
-done:
-    __syncwarp();
-    if (s_abort && warp == 4 * RING_GROUPS && lane == 0) {
-        // a wait gave up: give the copies already requested time to land before shared memory is released
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);
-    }
-    __syncthreads();
-}
-
-// ---------------------------------------------------------------------------------------
 // Many rows: 5th-generation tensor cores, accumulators in tensor memory
 // ---------------------------------------------------------------------------------------
 
@@ -724,27 +506,47 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
     const uint32_t full_lead = CG == 2 ? mapa_shared(bar_full, 0) : bar_full;
     if (warp == WARP_TMA) {
         if (lane == 0) {
-            const uint32_t bytes = CG * (GATHER ? Cfg::B_STAGE : Cfg::STAGE);
+            // this thread's instructions stand between a slot that is free and its copies: what does not change from stage to stage is
+            // formed once a tile
+            constexpr int PARTS = BN / CG < WT ? 1 : BN / CG / WT, HIGH = BN / CG < WT ? BN / CG : WT;  // tiles of weights a stage takes, their channels
+            const uint32_t a_smem = smem_u32(sA), b_smem = smem_u32(sB);
             uint32_t s = 0, ph = 1;
             for (int t = unit; t < tiles; t += units) {
                 const Tile c = tile_at(t);
                 const int n0 = c.n * BN + (int)rank * (BN / CG), m = c.m0 + (int)rank * BM;
+                // whole boxes that hold the tile's rows (what else the stage holds is multiplied and not stored); the first block counts both
+                auto boxes = [&](int first) { return GATHER ? 0 : min(max((c.last - first + p.q_box - 1) / p.q_box, 0), BM / p.q_box); };
+                const int mine = boxes(m), box_bytes = p.q_box * KCH;
+                const uint32_t bytes = CG * Cfg::B_STAGE + (uint32_t)((mine + (CG == 2 ? boxes(m + BM) : 0)) * box_bytes);
+                // a tile of channels past the last repeats the last one: its results are not stored
+                long long tile[PARTS];
+#pragma unroll
+                for (int n = 0; n < PARTS; n++) tile[n] = ((long long)c.e * p.n_tiles + min((n0 + n * WT) / WT, p.n_tiles - 1)) * p.k_tiles;
+                const int8_t* src[PARTS];
+                int w_row[PARTS];
+#pragma unroll
+                for (int n = 0; n < PARTS; n++) {
+                    src[n] = p.img + tile[n] * WT_BYTES + (n0 % WT) * KCH;
+                    w_row[n] = (int)(tile[n] * WT + n0 % WT);
+                }
                 for (int kt = 0; kt < p.k_tiles; kt++) {
                     if (!mbar_wait(bar_empty + 8 * s, ph, abort_flag, p.status, 1)) goto done;
-                    const uint32_t b_dst = smem_u32(sB + s * Cfg::B_STAGE), bar = full_lead + 8 * s;
+                    const uint32_t bar = full_lead + 8 * s, a_dst = a_smem + s * Cfg::A_STAGE, b_dst = b_smem + s * Cfg::B_STAGE;
                     if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
 #pragma unroll
-                    for (int n = 0; n < BN / CG; n += WT) {
-                        constexpr int HIGH = BN / CG < WT ? BN / CG : WT;
-                        const int nn = n0 + n;
-                        // a tile of channels past the last repeats the last one: its results are not stored
-                        const long long tile = ((long long)c.e * p.n_tiles + min(nn / WT, p.n_tiles - 1)) * p.k_tiles + kt;
-                        if (CG == 2) tma_tile2d_g2s_pair(b_dst + n * KCH, &maps.w, 0, (int)(tile * WT + nn % WT), bar);
-                        else bulk_g2s(b_dst + n * KCH, p.img + tile * WT_BYTES + (nn % WT) * KCH, HIGH * KCH, bar);
+                    for (int n = 0; n < PARTS; n++) {
+                        if (CG == 2) tma_tile2d_g2s_pair(b_dst + n * HIGH * KCH, &maps.w, 0, w_row[n], bar);
+                        else bulk_g2s(b_dst + n * HIGH * KCH, src[n], HIGH * KCH, bar);
+                        src[n] += WT_BYTES;
+                        w_row[n] += WT;
                     }
-                    if (!GATHER) {
-                        if (CG == 2) tma_tile2d_g2s_pair(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
-                        else tma_tile2d_g2s(smem_u32(sA + s * Cfg::A_STAGE), &maps.q, kt * KCH, m, bar);
+                    if (!GATHER && mine) {
+                        if (CG == 2) tma_tile2d_g2s_pair(a_dst, &maps.q, kt * KCH, m, bar);
+                        else tma_tile2d_g2s(a_dst, &maps.q, kt * KCH, m, bar);
+                        for (int i = 1; i < mine; i++) {
+                            if (CG == 2) tma_tile2d_g2s_pair(a_dst + i * box_bytes, &maps.q, kt * KCH, m + i * p.q_box, bar);
+                            else tma_tile2d_g2s(a_dst + i * box_bytes, &maps.q, kt * KCH, m + i * p.q_box, bar);
+                        }
                     }
                     if (++s == NSTG) { s = 0; ph ^= 1; }
                 }
@@ -938,7 +740,7 @@ template <int BN, int CG, bool GATHER>
 int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     using Cfg = TcI8<BN, CG, GATHER>;
     MapsI8 maps = {};
-    int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, BM, 128);
+    int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, a.q_box, 128);
     if (rc) return rc;
     // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
     if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;
@@ -958,20 +760,6 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     if (most * n_blocks >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many tiles: %d places of %d channels", a.places, a.N);
     const int grid = CG * (int)std::min<long long>(most * n_blocks, ctx->sm_count / CG);
     return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
-}
-
-template <int NT>
-int launch_few_ring(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
-    auto kern = gemm_i8_few_ring_kernel<NT>;
-    static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
-    if (!smem_set[ctx->device & 63]) {
-        TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring_few_smem(MAX_EXPERTS)));
-        smem_set[ctx->device & 63] = true;
-    }
-    const long long high = ((long long)a.places + 8 * NT - 1) / (8 * NT) + (a.offsets ? std::min(a.experts, a.places) : 0);  // at most
-    const long long items = high * ((a.N + RING_CH - 1) / RING_CH);
-    if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
-    return launch<GemmI8Args>(kern, ctx, (int)std::min<long long>(items, ctx->sm_count), RING_FEW_THREADS, ring_few_smem(a.experts), 1, stream, a);
 }
 
 // Warps that share the K tiles: at least four tiles a warp, so that their loads overlap, unless the pieces do not fill the SMs.
@@ -1009,17 +797,22 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const uintptr_t at = (uintptr_t)d_y | (uintptr_t)(y_stride * tnns_dtype_bytes(dtype));
     a.y_vec = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
     const cudaStream_t st = (cudaStream_t)stream;
-    // places an expert has on average
-    const long long rows = ((long long)places + w->experts - 1) / w->experts;
-    // pieces of the ring form: a block for every expert that has a row
-    const long long pieces = (long long)std::min(w->experts, places) * ((w->N + RING_CH - 1) / RING_CH);
-    const bool ring = d_offsets && pieces >= ctx->sm_count;
-    if (q_rows == 0 || rows <= 8) return ring ? launch_few_ring<1>(ctx, a, st) : launch_few<1>(ctx, a, st);
-    if (rows <= 16) return ring ? launch_few_ring<2>(ctx, a, st) : launch_few<2>(ctx, a, st);
-    const long long tiles = (long long)((places + 255) / 256) * ((w->N + 255) / 256);
-    // blocks of 128 rows: at least one for every expert that has a row
-    const long long high = std::max<long long>((places + 127) / 128, d_offsets ? std::min(w->experts, places) : 0);
-    if (tiles >= ctx->sm_count / 2 && rows > 128) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
+    // places an expert has on average, experts that may have one, pieces of 64 channels of those
+    const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);
+    const long long pieces = met * ((w->N + 63) / 64);
+    // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, tensor cores 14.9 / 10.8), or as many as make no more
+    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: where their
+    // weights do not fill the SMs with tiles (one token, 8 of 64 experts, 2048 -> 1024: 8.0 / 9.2 us; two tokens 10.8 / 9.9), or have one row each
+    // and short sums (8 tokens, 1024 -> 2048: 24.9 / 26.1 us; 2048 -> 1024 25.4 / 22.2).
+    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count || (rows <= 1 && w->k_tiles < 16);
+    if (q_rows == 0 || few) return rows <= 8 ? launch_few<1>(ctx, a, st) : launch_few<2>(ctx, a, st);
+    // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
+    // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).
+    a.q_box = rows <= 16 ? 32 : rows <= 64 ? 64 : BM;
+    // Block pairs where experts (or the one kernel) have more rows than a block, and there are tiles for every pair; else single blocks
+    // on tiles of 128 channels, or of 64 where those do not occupy half the SMs.
+    const long long pairs = ((long long)places + 255) / 256 * ((w->N + 255) / 256), high = std::max<long long>(((long long)places + 127) / 128, d_offsets ? met : 0);
+    if (rows > 128 && pairs >= ctx->sm_count / 2) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
     if (high * ((w->N + 127) / 128) >= ctx->sm_count / 2) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
     return d_rows ? launch_tc<64, 1, true>(ctx, a, st) : launch_tc<64, 1, false>(ctx, a, st);
 }

@@ -495,7 +495,7 @@ __device__ __forceinline__ void plan_pairs(const RouteArgs& p, const PlanArgs& o
     if (RANKS > 1) cluster_sync_all();  // no block leaves while another may read its counts
 }
 
-constexpr int ROUTE_WARPS = 16, PLAN_RANKS = 8, PLAN_THREADS = 1024;
+constexpr int ROUTE_WARPS = 16, PLAN_THREADS = 1024;
 
 // One warp a token.  PLAN: one block takes all tokens and orders the pairs as well.
 template <typename T, int NPL, bool PLAN>
@@ -517,12 +517,13 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, NPL <= 16 ? 2 : 1) route_ker
     }
 }
 
+template <int RANKS>
 __global__ void __launch_bounds__(PLAN_THREADS, 1) plan_kernel(const __grid_constant__ RouteArgs p, const __grid_constant__ PlanArgs o, int high) {
     extern __shared__ int s_plan[];
     __shared__ int s_part[32];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    plan_pairs<PLAN_RANKS, PLAN_THREADS>(p, o, high, s_plan, s_part, threadIdx.x);
+    plan_pairs<RANKS, PLAN_THREADS>(p, o, high, s_plan, s_part, threadIdx.x);
 }
 
 template <typename... Args>
@@ -565,19 +566,51 @@ int allow_smem(void (*kern)(Args...), size_t bytes, bool (&set)[64], int device)
     return TNNS_OK;
 }
 
+constexpr size_t PLAN_SMEM = 200 * 1024;
+template <int RANKS>
+int launch_plan_ranks(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, cudaStream_t st) {
+    static bool set[64] = {false};
+    const int rc = allow_smem(plan_kernel<RANKS>, PLAN_SMEM, set, ctx->device);
+    if (rc) return rc;
+    // groups of 32 tokens that a block holds at a time: all of its own, or as many as fit
+    const int own = (int)((((long long)a.T + 31) / 32 + RANKS - 1) / RANKS), fit = (int)((PLAN_SMEM / sizeof(int) / a.E - 4) / 2);
+    const int high = std::min(own, fit);
+    return launch<RouteArgs, PlanArgs, int>(plan_kernel<RANKS>, RANKS, PLAN_THREADS, plan_smem(high, a.E), RANKS, st, a, o, high);
+}
+// Clusters of sixteen blocks where the device takes them (its scattered stores bound the launch: 8192 tokens, 8 of 256 experts, eight blocks
+// 12.3 us, sixteen X), else of eight.
+int launch_plan(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, cudaStream_t st) {
+    static int ranks[64] = {0};
+    int& r = ranks[ctx->device & 63];
+    if (r == 0) {
+        r = 8;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        cfg.gridDim = dim3(16);
+        cfg.blockDim = dim3(PLAN_THREADS);
+        cfg.dynamicSmemBytes = PLAN_SMEM;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 16;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(plan_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+            cudaFuncSetAttribute(plan_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PLAN_SMEM) == cudaSuccess &&
+            cudaOccupancyMaxActiveClusters(&n, plan_kernel<16>, &cfg) == cudaSuccess && n > 0)
+            r = 16;
+        cudaGetLastError();  // a refusal is an answer here
+    }
+    return r == 16 ? launch_plan_ranks<16>(ctx, a, o, st) : launch_plan_ranks<8>(ctx, a, o, st);
+}
+
 template <typename T, int NPL>
 int launch_route(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, bool plan, cudaStream_t st) {
     int rc;
     if (plan && a.T <= ONE_BLOCK_TOKENS) return launch<RouteArgs, PlanArgs>(route_kernel<T, NPL, true>, 1, ROUTE_WARPS * 32, plan_smem(1, a.E), 1, st, a, o);
     const int blocks = std::min((a.T + ROUTE_WARPS - 1) / ROUTE_WARPS, (NPL <= 16 ? 2 : 1) * ctx->sm_count);
     if ((rc = launch<RouteArgs, PlanArgs>(route_kernel<T, NPL, false>, blocks, ROUTE_WARPS * 32, 0, 1, st, a, o)) || !plan) return rc;
-    static bool set[64] = {false};
-    constexpr size_t MOST = 200 * 1024;
-    if ((rc = allow_smem(plan_kernel, MOST, set, ctx->device))) return rc;
-    // groups of 32 tokens that a block holds at a time: all of its own, or as many as fit
-    const int own = (int)((((long long)a.T + 31) / 32 + PLAN_RANKS - 1) / PLAN_RANKS), fit = (int)((MOST / sizeof(int) / a.E - 4) / 2);
-    const int high = std::min(own, fit);
-    return launch<RouteArgs, PlanArgs, int>(plan_kernel, PLAN_RANKS, PLAN_THREADS, plan_smem(high, a.E), PLAN_RANKS, st, a, o, high);
+    return launch_plan(ctx, a, o, st);
 }
 // Registers a lane needs for its share of the experts.
 template <typename T>

@@ -50,8 +50,8 @@ __device__ __forceinline__ void realign(const uint4& a, const uint4& b, int off,
 }
 // Chunk i of a row of K elements, zeros past the row's end.  MIS: rows need not start on 16 bytes; the two aligned vectors that
 // overlap the chunk are fetched (the second only where it holds elements of the row, so that no other 16 bytes than those that
-// the row touches are read) and shifted together.
-template <typename T, bool MIS>
+// the row touches are read) and shifted together.  WHOLE: the caller knows that the chunk is complete.
+template <typename T, bool MIS, bool WHOLE = false>
 __device__ __forceinline__ Chunk<T> load_chunk(const T* row, int i, int K) {
     constexpr int VE = Chunk<T>::VE;
     Chunk<T> c;
@@ -63,11 +63,11 @@ __device__ __forceinline__ Chunk<T> load_chunk(const T* row, int i, int K) {
         const uint4* base = reinterpret_cast<const uint4*>((uintptr_t)row - off) + i;
         const uint4 a = base[0];
         uint4 b = make_uint4(0, 0, 0, 0);
-        if (off && ((long long)(i + 1) * 16 - off) < (long long)K * (int)sizeof(T)) b = base[1];
+        if (off && (WHOLE || ((long long)(i + 1) * 16 - off) < (long long)K * (int)sizeof(T))) b = base[1];
         realign<T>(a, b, off, c.w);
     }
     const int have = K - i * VE;
-    if (have < VE) {
+    if (!WHOLE && have < VE) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (sizeof(T) == 4) {
@@ -120,8 +120,9 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits, float* scale) {
 //                 1 / max((2n + 1) * A, 127 * X) > 2^-19 relative.  So r, rounded to 21 bits, is h exactly where the quotient is,
 //                 and on the quotient's side of h where it is not: no case is left.
 //   fp32          where r lies within 2^-15 of a half, x * 127 and h * a are compared in 64 bits, where both are exact.
-// Rows whose largest magnitude is too small for 127 / a to be a float divide in 64 bits.
-template <typename T, int VE>
+// Rows whose largest magnitude is too small for 127 / a to be a float divide in 64 bits.  PLAIN: the row is neither of those nor all
+// zeros.
+template <typename T, int VE, bool PLAIN>
 __device__ __forceinline__ void quantise_chunk(const float (&x)[VE], const RowScale& s, uint32_t (&out)[VE / 4]) {
     constexpr float MAGIC = 12582912.0f;
     uint32_t q[VE];
@@ -148,18 +149,18 @@ __device__ __forceinline__ void quantise_chunk(const float (&x)[VE], const RowSc
             }
         }
     }
-    if (s.exact) {
+    if (!PLAIN && s.exact) {
 #pragma unroll
         for (int j = 0; j < VE; j++) q[j] = (uint32_t)(int)rint((double)x[j] * 127.0 / (double)s.a);
     }
 #pragma unroll
-    for (int j = 0; j < VE / 4; j++) out[j] = s.zero ? 0u : __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
+    for (int j = 0; j < VE / 4; j++) out[j] = !PLAIN && s.zero ? 0u : __byte_perm(__byte_perm(q[4 * j], q[4 * j + 1], 0x0040), __byte_perm(q[4 * j + 2], q[4 * j + 3], 0x0040), 0x5410);
 }
-template <int VE>
+template <int VE, bool WHOLE>
 __device__ __forceinline__ void store_chunk(int8_t* out, int i, int K, const uint32_t (&q)[VE / 4]) {
     int8_t* at = out + (long long)i * VE;
     const int have = K - i * VE;
-    if (have >= VE) {
+    if (WHOLE || have >= VE) {
         if constexpr (VE == 8) *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
         else *reinterpret_cast<uint32_t*>(at) = q[0];
     } else {
@@ -169,14 +170,14 @@ __device__ __forceinline__ void store_chunk(int8_t* out, int i, int K, const uin
     }
 }
 
-template <typename T>
+template <typename T, bool WHOLE = false>
 __device__ __forceinline__ void finish_chunk(const Chunk<T>& c, int8_t* out, int i, int K, const RowScale& s) {
     constexpr int VE = Chunk<T>::VE;
     float f[VE];
     uint32_t w[VE / 4];
     unpack(c, f);
-    quantise_chunk<T, VE>(f, s, w);
-    store_chunk<VE>(out, i, K, w);
+    quantise_chunk<T, VE, WHOLE>(f, s, w);
+    store_chunk<VE, WHOLE>(out, i, K, w);
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const
     __shared__ uint64_t s_bar[RING_WARPS * RING_MAX_SLOTS];
     __shared__ int s_abort;
     constexpr int VE = Chunk<T>::VE;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (K + VE - 1) / VE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (K + VE - 1) / VE, whole = K / VE;
     const uint32_t bars = smem_u32(s_bar + warp * RING_MAX_SLOTS);
     unsigned char* ring = s_ring + (size_t)warp * slots * slot_bytes;
     if (threadIdx.x == 0) s_abort = 0;
@@ -265,12 +266,19 @@ __global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const
         }
         const T* row = reinterpret_cast<const T*>(ring + s * slot_bytes + (MIS ? (uintptr_t)(x + m * x_stride) & 15 : 0));
         uint32_t top = 0;
+        // (whole chunks without the tests that the last one needs)
 #pragma unroll 4
-        for (int i = lane; i < chunks; i += 32) top = widen_max(top, load_chunk<T, MIS>(row, i, K));
+        for (int i = lane; i < whole; i += 32) top = widen_max(top, load_chunk<T, MIS, true>(row, i, K));
+        if (whole < chunks && lane == 0) top = widen_max(top, load_chunk<T, MIS>(row, whole, K));
         const RowScale sc = row_scale(__reduce_max_sync(0xFFFFFFFFu, magnitude_bits<T>(top)), lane == 0 ? scale + m : nullptr);
         int8_t* out = q + m * q_stride;
-#pragma unroll 2
-        for (int i = lane; i < chunks; i += 32) finish_chunk(load_chunk<T, MIS>(row, i, K), out, i, K, sc);
+        if (sc.zero || sc.exact) {
+            for (int i = lane; i < chunks; i += 32) finish_chunk(load_chunk<T, MIS>(row, i, K), out, i, K, sc);
+        } else {
+#pragma unroll 4
+            for (int i = lane; i < whole; i += 32) finish_chunk<T, true>(load_chunk<T, MIS, true>(row, i, K), out, i, K, sc);
+            if (whole < chunks && lane == 0) finish_chunk(load_chunk<T, MIS>(row, whole, K), out, whole, K, sc);
+        }
         __syncwarp();
         if (lane == 0 && m + slots * step < M) {
             fence_async();  // the warp's reads before the copy's writes

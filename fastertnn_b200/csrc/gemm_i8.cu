@@ -809,11 +809,15 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
     // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).
     a.q_box = rows <= 16 ? 32 : rows <= 64 ? 64 : BM;
-    // Block pairs where experts (or the one kernel) have more rows than a block, and there are tiles for every pair; else single blocks
-    // on tiles of 128 channels, or of 64 where those do not occupy half the SMs.
-    const long long pairs = ((long long)places + 255) / 256 * ((w->N + 255) / 256), high = std::max<long long>(((long long)places + 127) / 128, d_offsets ? met : 0);
-    if (rows > 128 && pairs >= ctx->sm_count / 2) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
-    if (high * ((w->N + 127) / 128) >= ctx->sm_count / 2) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
+    // Tiles of 256 x 256 on block pairs, of 128 x 128 or of 128 x 64 on single blocks: what takes the fewest clocks, by the waves that the
+    // launch's tiles make and the clocks of a K tile in each (measured with every SM at work: about 620, 530 and 410; the large tiles
+    // are bound by the shared memory's bandwidth, the small ones by L2's).  1024 x 4096 -> 4096: pairs 17.6 us, 128 x 128 21.5; 512 rows 128 x
+    // 128 13.3, 128 x 64 18.6; 1024 x 4096 -> 1024: 128 x 64 11.3, 128 x 128 13.4.
+    const long long each = d_offsets ? met : 1;
+    auto clocks = [&](int tm, int tn, int units, int per_stage) { return ((rows + tm - 1) / tm * each * ((w->N + tn - 1) / tn) + units - 1) / units * per_stage; };
+    const long long pair = clocks(256, 256, ctx->sm_count / 2, 620), wide = clocks(128, 128, ctx->sm_count, 530), narrow = clocks(128, 64, ctx->sm_count, 410);
+    if (pair <= wide && pair <= narrow) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
+    if (wide <= narrow) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
     return d_rows ? launch_tc<64, 1, true>(ctx, a, st) : launch_tc<64, 1, false>(ctx, a, st);
 }
 

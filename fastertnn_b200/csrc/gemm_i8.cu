@@ -112,7 +112,7 @@ __device__ __forceinline__ int expert_of(const int* s_first, int experts, int b)
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows: the weights are read once, straight into the operand registers of the warp-level matrix instruction
+// Few rows: the weights go straight into the operand registers of the warp-level matrix instruction
 // ---------------------------------------------------------------------------------------
 
 constexpr int FEW_WARPS = 8;
@@ -138,7 +138,8 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 // such pieces side by side and goes on to others, whose weights it requests before it finishes the present ones.  Bounded by the
 // weights' bytes: a lane (g, t) holds the 32 bytes of pieces 2t and 2t + 1 of channels 2g and 2g + 1 (rows g and g + 8 of the
 // instruction), so a load takes eight whole lines, four instructions multiply a K tile of 2 KB, and no byte passes through shared
-// memory.  The order of K within the tile is the same for weights and rows.
+// memory.  The order of K within the tile is the same for weights and rows.  1 x 4096 -> 4096: 5.0 us = 3.4 TB/s, of which the launch and
+// the first bytes' way take 2.4.
 template <int NT>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int log_s) {
     constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
@@ -340,9 +341,10 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
 // 64 bytes of each of a warp's rows to y: w = those of the lane's row; they leave through the warp's 32 x 64 bytes of shared memory,
 // the 16-byte pieces of a row in the pattern piece ^ (row / 2) % 4 (the copy engine's 64-byte swizzle, free of bank conflicts).
 // Whole blocks go out as one tensor copy where y allows it (vec >= 16: bytes that may be stored at once everywhere in y; a copy that
-// ends inside 16 bytes of a row would write all of them).  A store by lanes, each 32 bytes of its own row, took 32 bytes a clock off the path that also feeds the tensor core: 65536 x
-// 1024 -> 2048 in 134 us against X.  The rest the warp writes along the rows.  x, row0: first byte of the row, first row; have: bytes
-// of a row that exist (a multiple of `size`, an element's bytes); step: bytes from row to row.
+// ends inside 16 bytes of a row would write all of them).  A store by lanes, each 32 bytes of its own row, took 32 bytes a clock off the
+// path that also feeds the tensor core: 65536 x 1024 -> 2048 bf16 in 134 us against 118, fp32 177 against 143.  The rest the warp writes
+// along the rows (4096 x 1024 -> 4097: 39 us, by lanes 190).  x, row0: first byte of the row, first row; have: bytes of a row that exist
+// (a multiple of `size`, an element's bytes); step: bytes from row to row.
 __device__ __forceinline__ void store_rows(const uint32_t (&w)[16], uint32_t* stage, const void* tmap, unsigned char* base, int x, int row0, long long step, int rows,
                                            int have, int vec, int size, int lane) {
     auto at = [&](int row, int word) { return stage + row * 16 + ((((word >> 2) ^ (row >> 1)) & 3) << 2) + (word & 3); };
@@ -424,9 +426,13 @@ __device__ __forceinline__ void finish_words(int dtype, const uint32_t* v, float
 
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
 // of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
-// MMAs, warps 2 to 7 gather rows where places name them (each a slot of the ring, so that all are on their way at once), warps 8 to 15
-// scale, round and store one accumulator while the MMAs fill the other.  Gathering through the copy engine, four rows a request,
-// was measured first: 80 clocks a request of 512 bytes, 360 us where the warps take X (8192 tokens, 8 of 64 experts, 2048 -> 1024).
+// MMAs, where places name their rows six warps gather them (each a slot of the ring, so that all are on their way at once), and sixteen
+// (tiles of 64 channels: eight) scale, round and store one accumulator while the MMAs fill the other.
+// Large products are bound by the tensor pipe at the clock that the power limit leaves: 8192 x 4096 -> 8192 in 170 us, 3.2 POP/s, 0.98 of
+// twice the measured bf16 rate (its pipe 75 % active by count: operands come in and go to the pipe at 127 of the shared memory's 128
+// bytes a clock).  Short sums are bound by what their results add to that path: 65536 x 1024 -> 2048 118 us, 82 without results.
+// Rows by gathering tensor copies, four a request, took 80 clocks a request of 512 bytes: 8192 tokens by 8 of 64 experts, 2048 -> 1024, 360
+// us against 128 by the warps.
 template <int BN, int CG, bool GATHER>
 __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_kernel(const __grid_constant__ GemmI8Args p, const __grid_constant__ MapsI8 maps) {
     using Cfg = TcI8<BN, CG, GATHER>;

@@ -578,7 +578,7 @@ int launch_plan_ranks(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o,
     return launch<RouteArgs, PlanArgs, int>(plan_kernel<RANKS>, RANKS, PLAN_THREADS, plan_smem(high, a.E), RANKS, st, a, o, high);
 }
 // Clusters of sixteen blocks where the device takes them (its scattered stores bound the launch: 8192 tokens, 8 of 256 experts, eight blocks
-// 12.3 us, sixteen X), else of eight.
+// 12.3 us, sixteen 10.1), else of eight.
 int launch_plan(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, cudaStream_t st) {
     static int ranks[64] = {0};
     int& r = ranks[ctx->device & 63];

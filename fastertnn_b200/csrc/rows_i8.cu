@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
 
 // Many rows: persistent blocks, RING_WARPS warps, each with rows of its own that the copy engine brings into its slots of shared
 // memory (the aligned 16 bytes that the row touches), `slots` a warp, ahead of the warp's work: the bytes on their way do not
-// depend on registers.  A warp goes over its row twice, for the largest magnitude and for the integers.
+// depend on registers.  A warp goes over its row twice, for the largest magnitude and for the integers.  Bounded by memory for fp32 (8192 x
+// 4096: 31 us = 5.4 TB/s, 0.82 of the measured copy; rows in registers 45), by instructions for 16-bit types (19.6 us = 5.1 TB/s;
+// rows in registers 33) and short rows (20000 x 512 bf16: 12.4 us).
 constexpr int RING_WARPS = 12, RING_MAX_SLOTS = 8, RING_BYTES = 200 * 1024;
 template <typename T, bool MIS>
 __global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const T* __restrict__ x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
@@ -388,7 +390,7 @@ __device__ __forceinline__ void store_sums(const CombineArgs& p, long long row, 
 }
 
 // One thread a chunk of VE neighbouring columns (16 bytes of y) of a token, the rows of eight slots on their way at once.  Bounded by
-// memory: every row of y is read once.  MIS: rows need not start on 16 bytes; the first chunk of a row begins where its results are
+// memory: every row of y is read once (8192 tokens of 8 x 2048 bf16: 54 us = 5.6 TB/s, 0.86 of the measured copy; rows of 2047: 101 us).  MIS: rows need not start on 16 bytes; the first chunk of a row begins where its results are
 // aligned (at a column up to VE - 1 below 0), and y is fetched as the aligned vectors that hold the chunk.
 template <typename T, bool MIS>
 __global__ void __launch_bounds__(256) combine_kernel(CombineArgs p) {

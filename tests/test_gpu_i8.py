@@ -1,5 +1,9 @@
 """GPU suite: rows to 8-bit integers, their products with 8-bit weights (dense and by expert), and the sum back to the tokens,
 against the definitions in 64 bits."""
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -525,6 +529,35 @@ def test_layer_captured_and_replayed(T, E, k, D, H, gpu_ctx):
         layer.free()
 
 
+FIRST_CALLS = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+import fastertnn_b200 as ft
+from test_gpu_i8 import Layer, gen
+ctx = ft.Context(0)
+for T, E, k, D, H in ((5, 16, 4, 256, 128), (300, 16, 4, 2048, 1024), (5000, 16, 4, 384, 640)):
+    layer = Layer(ctx, T, E, k, D, H, T)
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        layer.run(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    ctx.sync()
+    layer.check()
+print("all captured")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of every kernel is made while a stream is captured."""
+    here = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS % (str(here), str(here.parent))], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "all captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_results_do_not_change_from_run_to_run(gpu_ctx):
     layer = Layer(gpu_ctx, 513, 16, 4, 512, 256, 5)
     layer.run(stream())
@@ -554,6 +587,27 @@ def test_behind_a_slow_producer(gpu_ctx):
     st.synchronize()
     layer.check()
     layer.free()
+
+
+def test_outputs_of_one_call_as_inputs_of_the_next_without_a_pause(gpu_ctx):
+    """Products in a row on one stream, each reading what the one before wrote (launches may overlap up to their waits)."""
+    g = gen(21)
+    D, M = 512, 300
+    w, s = int8(g, D, D), torch.rand(D, generator=g) * 1e-3
+    h = gpu_ctx.upload_weights_i8(w.data_ptr(), s.data_ptr(), D, D)
+    x = torch.randn(M, D, generator=g).cuda()
+    for rows in (1, 40, M):
+        q, sc = torch.empty(rows, D, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+        a = [x[:rows].clone()] + [torch.empty(rows, D, device="cuda") for _ in range(12)]
+        for i in range(12):
+            gpu_ctx.quantise_i8(a[i].data_ptr(), ft.F32, q.data_ptr(), sc.data_ptr(), rows, D, stream=stream())
+            gpu_ctx.gemm_i8(h, q.data_ptr(), sc.data_ptr(), a[i + 1].data_ptr(), ft.F32, rows, 0.5, stream=stream())
+        gpu_ctx.sync()
+        for i in range(12):
+            qq, ss = quantise(a[i])
+            want = product(qq, ss, w.numpy(), s.numpy(), 0.5)
+            assert (np.abs(f64(a[i + 1]) - want) <= product_error(want, "f32")).all()
+    h.free()
 
 
 def test_on_a_second_device(gpu_ctx):

@@ -807,10 +807,10 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);
     const long long pieces = met * ((w->N + 63) / 64);
     // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, tensor cores 14.9 / 10.8), or as many as make no more
-    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: where their
-    // weights do not fill the SMs with tiles (one token, 8 of 64 experts, 2048 -> 1024: 8.0 / 9.2 us; two tokens 10.8 / 9.9), or have one row each
-    // and short sums (8 tokens, 1024 -> 2048: 24.9 / 26.1 us; 2048 -> 1024 25.4 / 22.2).
-    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count || (rows <= 1 && w->k_tiles < 16);
+    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: where those that have
+    // a row make fewer pieces than SMs (one token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two tokens 10.8 / 9.9; eight, 1024
+    // -> 2048: 24.8 / 20.5).
+    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count;
     if (q_rows == 0 || few) return rows <= 8 ? launch_few<1>(ctx, a, st) : launch_few<2>(ctx, a, st);
     // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
     // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).

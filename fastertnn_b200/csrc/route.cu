@@ -20,9 +20,10 @@ struct RouteArgs {
     float scale;
 };
 
-// A logit or a bias that bars its expert: -inf and NaN.  +inf counts as the largest finite float.
+// A logit or a bias as it counts: -inf and NaN bar its expert (-inf: a maximum returns the operand that is a number), +inf is the
+// largest finite float.
+__device__ __forceinline__ float bounded(float v) { return fminf(fmaxf(v, -INFINITY), 3.402823466e38f); }
 __device__ __forceinline__ bool barred(float v) { return !(v > -INFINITY); }
-__device__ __forceinline__ float bounded(float v) { return fminf(v, 3.402823466e38f); }
 
 constexpr int MAX_E = 1024;
 constexpr unsigned FULL = 0xFFFFFFFFu;
@@ -83,6 +84,12 @@ __device__ __forceinline__ double warp_max(double v) {
     b ^= (b >> 63) & 0x7FFFFFFFFFFFFFFFLL;
     return __longlong_as_double(b);
 }
+// 2^(v log2 e), off by 2^-22 and by the rounding of the product
+__device__ __forceinline__ float exponential(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.44269504f));
+    return r;
+}
 __device__ __forceinline__ float reciprocal(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -90,7 +97,7 @@ __device__ __forceinline__ float reciprocal(float v) {
 }
 // A score in fp32 by the fast exponential and quotient, or in 64 bits.
 __device__ __forceinline__ float score_of(const RouteArgs& p, float l, float top, float all) {
-    return p.sigmoid ? reciprocal(1.0f + __expf(-l)) : __expf(l - top) * reciprocal(all);
+    return p.sigmoid ? reciprocal(1.0f + exponential(-l)) : exponential(l - top) * reciprocal(all);
 }
 __device__ __forceinline__ double score_of(const RouteArgs& p, double l, double top, double all) {
     return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / all;
@@ -227,7 +234,7 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
     float top = -INFINITY;
 #pragma unroll
     for (int r = 0; r < NPL; r++) {
-        key[r] = barred(key[r]) ? -INFINITY : bounded(key[r]);
+        key[r] = bounded(key[r]);
         top = fmaxf(top, key[r]);
     }
     c.top = c.sum = 0.f;
@@ -236,7 +243,7 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
         if (c.top > -INFINITY) {
             float sum = 0.f;
 #pragma unroll
-            for (int r = 0; r < NPL; r++) sum += __expf(key[r] - c.top);  // exp(-inf) = 0
+            for (int r = 0; r < NPL; r++) sum += exponential(key[r] - c.top);  // exp(-inf) = 0
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(FULL, sum, d);
             c.sum = sum;
         }
@@ -247,8 +254,8 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
         const float inverse = reciprocal(c.sum);
 #pragma unroll
         for (int r = 0; r < NPL; r++) {
-            const float s = p.sigmoid ? reciprocal(1.0f + __expf(-key[r])) : __expf(key[r] - c.top) * inverse;
-            key[r] = key[r] == -INFINITY || barred(b[r]) ? -INFINITY : s + bounded(b[r]);
+            const float s = p.sigmoid ? reciprocal(1.0f + exponential(-key[r])) : exponential(key[r] - c.top) * inverse;
+            key[r] = key[r] == -INFINITY ? -INFINITY : s + bounded(b[r]);  // (-inf where the bias is)
         }
     }
     // the register's number: a larger one makes a key smaller, whatever its sign; infinity keeps its bits
@@ -577,8 +584,8 @@ int launch_plan_ranks(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o,
     const int high = std::min(own, fit);
     return launch<RouteArgs, PlanArgs, int>(plan_kernel<RANKS>, RANKS, PLAN_THREADS, plan_smem(high, a.E), RANKS, st, a, o, high);
 }
-// Clusters of sixteen blocks where the device takes them (its scattered stores bound the launch: 8192 tokens, 8 of 256 experts, eight blocks
-// 12.3 us, sixteen 10.1), else of eight.
+// Clusters of sixteen blocks where the device takes them (the blocks' shared-memory counts and scattered stores bound the launch: 8192
+// tokens, 8 of 256 experts, eight blocks 12.3 us, sixteen 10.1), else of eight.
 int launch_plan(tnns_cuda_ctx* ctx, const RouteArgs& a, const PlanArgs& o, cudaStream_t st) {
     static int ranks[64] = {0};
     int& r = ranks[ctx->device & 63];

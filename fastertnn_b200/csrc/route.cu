@@ -186,22 +186,22 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
     return mine;
 }
 
+// A softmax's sum in 64 bits, by the whole warp.
+template <typename T>
+__device__ __forceinline__ double exact_sum(const RouteArgs& p, const T* row, int lane, double top) {
+    double all = 0;
+    for (int e = lane; e < p.E; e += 32) {
+        const float v = to_f32(row[e]);
+        if (!barred(v)) all += exp((double)bounded(v) - top);
+    }
+    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(FULL, all, d);
+    return all;
+}
 // The candidates' order in 64 bits: lane j < n has expert `mine` (MAX_E: none) of logit l and bias b.  Returns the expert of place j.
 template <typename T>
 __device__ __noinline__ int order_exact(const RouteArgs& p, const T* row, int lane, int n, int mine, float l, float b, float top) {
     double key = (double)bounded(l);
-    if (p.bias) {
-        double all = 1;
-        if (!p.sigmoid) {
-            all = 0;
-            for (int e = lane; e < p.E; e += 32) {
-                const float v = to_f32(row[e]);
-                if (!barred(v)) all += exp((double)bounded(v) - (double)top);
-            }
-            for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(FULL, all, d);
-        }
-        key = score_of(p, key, (double)top, all) + (double)bounded(b);
-    }
+    if (p.bias) key = score_of(p, key, (double)top, p.sigmoid ? 1.0 : exact_sum(p, row, lane, (double)top)) + (double)bounded(b);
     int place = 0, result = MAX_E;
     for (int i = 0; i < n; i++) {
         const double o = __shfl_sync(FULL, key, i);
@@ -214,12 +214,34 @@ __device__ __noinline__ int order_exact(const RouteArgs& p, const T* row, int la
     }
     return result;
 }
+// Whether the lane's group is among the best, in 64 bits: ea, eb are the lane's two best experts (MAX_E: none).
+template <typename T>
+__device__ __noinline__ bool groups_exact(const RouteArgs& p, const T* row, int lane, int ea, int eb, float top) {
+    const Lanes at(p, lane);
+    const bool by_logit = p.group_top == 1 && !p.bias;
+    const double all = p.sigmoid || by_logit ? 1.0 : exact_sum(p, row, lane, (double)top);
+    double v[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int e = i ? eb : ea;
+        v[i] = -INFINITY;
+        if (e < MAX_E) {
+            const double l = (double)bounded(to_f32(row[e]));
+            v[i] = by_logit ? l : score_of(p, l, (double)top, all) + (p.bias ? (double)bounded(__ldg(p.bias + e)) : 0.0);
+        }
+    }
+    __syncwarp();
+    bool kept;
+    rank_group<double>(p, at, fmax(v[0], v[1]), fmin(v[0], v[1]), kept);
+    return kept;
+}
 
 // The choice for one token by one warp, in fp32.  Every lane sorts its keys, and the warp takes the best of the lanes' first ones,
 // top_k times.  A key carries its register's number in its lowest bits (LOG of them), lower registers above higher ones.
 //
-// That is certain unless two keys that have to be told apart are closer than their errors.  Experts that are near each other are then
-// ordered in 64 bits, and a token whose groups are is chosen in 64 bits altogether.  A score by the fast functions is off by 2^-22 from the exponential and by the rounding of its argument, of which a score (at
+// That is certain unless two keys that have to be told apart are closer than their errors.  Experts, or groups, that are near each other
+// are then ordered in 64 bits by themselves; where that is not enough (a lane's third best near its second, more candidates than lanes)
+// the token is chosen in 64 bits altogether.  A score by the fast functions is off by 2^-22 from the exponential and by the rounding of its argument, of which a score (at
 // most 1, and s * d <= 1 / e) keeps 2^-22 together; a softmax's sum adds NPL + 5 roundings of 2^-24, the quotient 2^-22, the bias
 // |key| * 2^-24.  A key without a bias is the logit itself.  The register's number takes LOG bits.  Two keys are in order if they
 // differ by (NPL + 24) * 2^-23 + |key| * 2^(LOG - 21) (first term: with a bias), or if they are made of the same logit and the same
@@ -296,7 +318,12 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
         // (a score made of a logit that lost LOG bits is off by |logit| times that; s * |logit| <= s * |top| + 1 / e)
         const float lost = sums ? (1.0f + (p.sigmoid ? 0.f : fabsf(c.top) * fabsf(worst_in))) * tol1 : 0.f;
         const float tol = 2 * ((NPL + 24) * 0x1p-23f * (p.bias || sums) + fmaxf(fabsf(worst_in), fabsf(best_out)) * (tol1 + 0x1p-22f) + lost) + 1e-30f;  // (a worth is made of two)
-        certain = best_out == -INFINITY || worst_in - best_out > tol;
+        if (!(best_out == -INFINITY || worst_in - best_out > tol)) {
+            // the lanes' two best are certain as such unless a third is near them
+            const bool third = NPL > 2 && key[1] != -INFINITY && key[NPL > 2 ? 2 : 1] != -INFINITY && near(key[1], key[NPL > 2 ? 2 : 1]);
+            if (__any_sync(FULL, third)) certain = false;
+            else kept = groups_exact<T>(p, row, lane, key[0] == -INFINITY ? MAX_E : at.e0 + register_of(key[0]), key[1] == -INFINITY ? MAX_E : at.e0 + register_of(key[1]), c.top);
+        }
         if (!kept) key[0] = -INFINITY;
     }
     // lane j < n: the j-th best key and its expert

@@ -107,6 +107,26 @@ def test_near_ties(groups, top_groups, gap, score, gpu_ctx):
     check(gpu_ctx, ft.Route(E, k, score, groups, top_groups, 2, 1, 1.0), logits[torch.from_numpy(fine)], bias)
 
 
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("middle", [0.0, 17.0, 40.0, -30.0, 1000.0])
+@pytest.mark.parametrize("E,groups,top_groups", [(128, 8, 3), (256, 4, 1), (60, 5, 2), (32, 1, 1)])
+def test_logits_next_to_each_other(E, groups, top_groups, middle, group_top, score, gpu_ctx):
+    """Logits that differ in their last bits only, where scores are steep and where they are all alike."""
+    logits = middle + torch.randint(-3, 4, (150, E), generator=gen(E)) * max(abs(middle), 1.0) * 2.0 ** -23
+    logits[::3] += torch.randint(0, 2, (50, E), generator=gen(E + 1)) * 0.5
+    if score == 0 and group_top == 2:  # sums of a softmax's scores that differ by less than 64-bit arithmetic rounds have no defined order
+        x = f64(logits)
+        p = np.exp(x - x.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        worth = np.sort(np.sort(p.reshape(150, groups, -1), 2)[:, :, -2:].sum(2), 1)
+        gaps = np.diff(worth, axis=1)
+        logits = logits[torch.from_numpy(((gaps > 1e-14) | (gaps == 0)).all(1))]
+        if not len(logits):
+            pytest.skip("no row with a defined order")
+    check(gpu_ctx, ft.Route(E, 6, score, groups, top_groups, group_top, 1, 1.0), logits.float())
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("with_bias", [False, True])
 @pytest.mark.parametrize("score", [0, 1])

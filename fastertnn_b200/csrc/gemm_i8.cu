@@ -343,7 +343,7 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
 // Whole blocks go out as one tensor copy where y allows it (vec >= 16: bytes that may be stored at once everywhere in y; a copy that
 // ends inside 16 bytes of a row would write all of them).  A store by lanes, each 32 bytes of its own row, took 32 bytes a clock off the
 // path that also feeds the tensor core: 65536 x 1024 -> 2048 bf16 in 134 us against 118, fp32 177 against 143.  The rest the warp writes
-// along the rows (4096 x 1024 -> 4097: 39 us, by lanes 190).  x, row0: first byte of the row, first row; have: bytes of a row that exist
+// along the rows (4096 x 1024 -> 4097: 37 us, by lanes 190).  x, row0: first byte of the row, first row; have: bytes of a row that exist
 // (a multiple of `size`, an element's bytes); step: bytes from row to row.
 __device__ __forceinline__ void store_rows(const uint32_t (&w)[16], uint32_t* stage, const void* tmap, unsigned char* base, int x, int row0, long long step, int rows,
                                            int have, int vec, int size, int lane) {
@@ -363,22 +363,27 @@ __device__ __forceinline__ void store_rows(const uint32_t (&w)[16], uint32_t* st
         return;
     }
     __syncwarp();
-    // half a warp a row
-    const int col = lane & 15;
-    unsigned char* y = base + (long long)(row0 + (lane >> 4)) * step + x;
-    for (int r0 = 0; r0 < rows; r0 += 2, y += 2 * step) {
-        const int r = r0 + (lane >> 4);
-        const uint32_t v = *at(r, col), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
-        if (r >= rows) continue;
-        if (size == 4 || (reinterpret_cast<uintptr_t>(y) & 2) == 0) {
+    // half a warp a row; rows that all start on a word without a neighbour's half (one loop for both kinds: 11364 x 129 -> 2118 39.8 us against 32.9)
+    const int col = lane & 15, half = lane >> 4;
+    unsigned char* y = base + (long long)(row0 + half) * step + x;
+    if (size == 4 || ((reinterpret_cast<uintptr_t>(base) | step) & 2) == 0) {
+        for (int r = half; r < rows; r += 2, y += 2 * step) {
+            const uint32_t v = *at(r, col);
             if (4 * col + 4 <= have) *reinterpret_cast<uint32_t*>(y + 4 * col) = v;
             else if (4 * col + 2 <= have) *reinterpret_cast<uint16_t*>(y + 4 * col) = (uint16_t)v;
-        } else {
-            // a row that starts between two words: the halves of neighbours together, the first and the last by themselves
-            if (col == 0) *reinterpret_cast<uint16_t*>(y) = (uint16_t)v;
-            if (4 * col + 6 <= have) *reinterpret_cast<uint32_t*>(y + 2 + 4 * col) = __funnelshift_r(v, next, 16);
-            else if (4 * col + 4 <= have) *reinterpret_cast<uint16_t*>(y + 2 + 4 * col) = (uint16_t)(v >> 16);
         }
+        return;
+    }
+#pragma unroll 4
+    for (int r0 = 0; r0 < 32; r0 += 2, y += 2 * step) {
+        const bool there = r0 + half < rows, odd = reinterpret_cast<uintptr_t>(y) & 2;
+        const uint32_t v = *at(r0 + half, col), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+        // a row that starts between two words: the halves of neighbours together, the first and the last by themselves
+        const int from = odd ? 2 : 0;  // the lane's word begins so many bytes behind its own column
+        const uint32_t w4 = odd ? __funnelshift_r(v, next, 16) : v;
+        if (there && 4 * col + 4 + from <= have) *reinterpret_cast<uint32_t*>(y + 4 * col + from) = w4;
+        else if (there && 4 * col + 2 + from <= have) *reinterpret_cast<uint16_t*>(y + 4 * col + from) = (uint16_t)w4;
+        if (there && odd && col == 0) *reinterpret_cast<uint16_t*>(y) = (uint16_t)v;
     }
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -807,10 +812,10 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);
     const long long pieces = met * ((w->N + 63) / 64);
     // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, tensor cores 14.9 / 10.8), or as many as make no more
-    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: where those that have
-    // a row make fewer pieces than SMs (one token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two tokens 10.8 / 9.9; eight, 1024
-    // -> 2048: 24.8 / 20.5).
-    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count;
+    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: up to 32
+    // rows each, where those that have a row make fewer pieces than SMs (one token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two
+    // tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8 experts, 1561 -> 226: 27 / 10.6).
+    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count && rows <= 32;
     if (q_rows == 0 || few) return rows <= 8 ? launch_few<1>(ctx, a, st) : launch_few<2>(ctx, a, st);
     // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
     // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).

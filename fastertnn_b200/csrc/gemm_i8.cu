@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __
 
 // Stages of 128 bytes of K: 128 rows of q (one tensor copy, or 16-byte copies by the gather warps where places name their rows) and
 // BN / CG channels of weights (contiguous copies of the tiled image).
-template <int BN, int CG, bool GATHER>
+template <int BN, int CG, bool GATHER, int CS>
 struct TcI8 {
     static constexpr int A_STAGE = BM * KCH, B_STAGE = BN / CG * KCH, STAGE = A_STAGE + B_STAGE;
     static constexpr int NSTG = 5 * 32768 / STAGE;
@@ -298,7 +298,10 @@ struct TcI8 {
     static constexpr int EPI_WARPS = BN == 64 ? 8 : 16, HN = BN / (EPI_WARPS / 4), THREADS = 32 * (EPI0 + EPI_WARPS);  // HN: channels of an epilogue warp
     static constexpr int BARS = 2 * NSTG + 2 * NBUF;
     static constexpr int STAGED = 16;  // words of a row of a warp's buffer for results on their way out
-    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + EPI_WARPS * (32 * STAGED + HN) * 4 + list_bytes(experts); }
+    static constexpr int SHARED_SUMS = (CS - 1) * (BN / CS) * BM;  // words that the cluster's other blocks send
+    static constexpr int OUT = EPI_WARPS * 32 * STAGED > SHARED_SUMS ? EPI_WARPS * 32 * STAGED : SHARED_SUMS;
+    static constexpr size_t smem(int experts) { return 1024 + (size_t)NSTG * STAGE + 8 * BARS + 16 + (OUT + EPI_WARPS * HN) * 4 + list_bytes(experts); }
+    static_assert(CS == 1 || (CG == 1 && !GATHER && HN == 32 && BN % (32 * CS) == 0), "shares: single blocks, whole warps of channels");
     static_assert(!GATHER || NSTG <= GATHER_WARPS, "a gather warp for every slot");
 };
 struct alignas(64) MapsI8 {
@@ -429,6 +432,27 @@ __device__ __forceinline__ void finish_words(int dtype, const uint32_t* v, float
     }
 }
 
+// 32 x 32 accumulators of a warp, from place place0 and channel n on: scaled, rounded and stored.
+__device__ __forceinline__ void store_chunk(const GemmI8Args& p, const MapsI8& maps, const uint32_t (&v)[32], float rs, const float* ws, int mode, uint32_t* stage, int n,
+                                            int place0, int rows, int size, int lane) {
+    const int have = (p.N - n) * size, x = n * size;
+    if (rows <= 0 || have <= 0) return;
+    const long long step = p.y_stride * size;
+    unsigned char* base = reinterpret_cast<unsigned char*>(p.y);
+    uint32_t w[16];
+    if (size == 4) {
+        finish_words<16>(p.dtype, v, rs, ws, p.alpha, mode, w);
+        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_vec, 4, lane);
+        if (have > 64) {
+            finish_words<16>(p.dtype, v + 16, rs, ws + 16, p.alpha, mode, w);
+            store_rows(w, stage, &maps.y, base, x + 64, place0, step, rows, min(have - 64, 64), p.y_vec, 4, lane);
+        }
+    } else {
+        finish_words<32>(p.dtype, v, rs, ws, p.alpha, mode, w);
+        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_vec, 2, lane);
+    }
+}
+
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
 // of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
 // MMAs, where places name their rows six warps gather them (each a slot of the ring, so that all are on their way at once), and sixteen
@@ -438,9 +462,14 @@ __device__ __forceinline__ void finish_words(int dtype, const uint32_t* v, float
 // bytes a clock).  Short sums are bound by what their results add to that path: 65536 x 1024 -> 2048 118 us, 82 without results.
 // Rows by gathering tensor copies, four a request, took 80 clocks a request of 512 bytes: 8192 tokens by 8 of 64 experts, 2048 -> 1024, 360
 // us against 128 by the warps.
-template <int BN, int CG, bool GATHER>
-__global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_kernel(const __grid_constant__ GemmI8Args p, const __grid_constant__ MapsI8 maps) {
-    using Cfg = TcI8<BN, CG, GATHER>;
+//
+// Where tiles are few and K is long, a cluster of CS blocks shares a tile (one a cluster): each multiplies its part of the K tiles, sends
+// the sums of the channels that others finish into their shared memory, adds what comes to its own 1 / CS of the channels and finishes
+// those.  Sums of integers: the result is the same whichever blocks form it.  The exchange (a cluster's start, its barrier, 16 KB from
+// each block for every 32 channels of another) takes about 2.5 us, a K tile of a lone block 0.2: 128 x 8192 -> 2048 17.7 us alone, 11.0 by four.
+template <int BN, int CG, bool GATHER, int CS = 1>
+__global__ void __launch_bounds__(TcI8<BN, CG, GATHER, CS>::THREADS, 1) gemm_i8_tc_kernel(const __grid_constant__ GemmI8Args p, const __grid_constant__ MapsI8 maps) {
+    using Cfg = TcI8<BN, CG, GATHER, CS>;
     constexpr int NSTG = Cfg::NSTG, NBUF = Cfg::NBUF, TM = CG * BM;
     // s32 accumulators, signed 8-bit operands, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
     constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
@@ -448,7 +477,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *sA = smem, *sB = smem + NSTG * Cfg::A_STAGE;
     uint32_t* s_stage = reinterpret_cast<uint32_t*>(smem + NSTG * Cfg::STAGE);              // [epilogue warp][32][STAGED]
-    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::EPI_WARPS * 32 * Cfg::STAGED);    // [epilogue warp][HN]: its channels' scales
+    float* s_ws = reinterpret_cast<float*>(s_stage + Cfg::OUT);                               // [epilogue warp][HN]: its channels' scales
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_ws + Cfg::EPI_WARPS * Cfg::HN);
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * NSTG, bar_tfull = bar_empty + 8 * NSTG, bar_tempty = bar_tfull + 8 * NBUF;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::BARS);
@@ -457,7 +486,15 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
-    const int unit = blockIdx.x / CG, units = gridDim.x / CG;
+    const int unit = blockIdx.x / (CG * CS), units = gridDim.x / (CG * CS);
+    const int share = CS > 1 ? (int)cluster_ctarank() : 0, k0 = p.k_tiles * share / CS, k1 = p.k_tiles * (share + 1) / CS;  // the block's K tiles
+    float share_rs = 0.f;
+    // OWN chunks of 32 channels are the block's to finish.  4 KB for a warp's chunk from each of the other blocks, those of one warp together;
+    // 16 bytes a lane, so that a warp's are next to each other.
+    constexpr int OWN = BN >= 32 * CS ? BN / 32 / CS : 1;
+    auto sums_at = [&](int chunk, int q, int from) {
+        return smem_u32(s_stage) + (((chunk % OWN) * 4 + q) * (CS - 1) + (from - chunk / OWN - 1 + CS) % CS) * 4096 + lane * 16;
+    };
 
     if (tid == 0) {
         for (int s = 0; s < NSTG; s++) {
@@ -485,7 +522,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     tc_fence_before();
-    if (CG == 2) cluster_sync_all(); else __syncthreads();
+    if (CG * CS > 1) cluster_sync_all(); else __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -537,10 +574,10 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
                 int w_row[PARTS];
 #pragma unroll
                 for (int n = 0; n < PARTS; n++) {
-                    src[n] = p.img + tile[n] * WT_BYTES + (n0 % WT) * KCH;
+                    src[n] = p.img + (tile[n] + k0) * WT_BYTES + (n0 % WT) * KCH;
                     w_row[n] = (int)(tile[n] * WT + n0 % WT);
                 }
-                for (int kt = 0; kt < p.k_tiles; kt++) {
+                for (int kt = k0; kt < k1; kt++) {
                     if (!mbar_wait(bar_empty + 8 * s, ph, abort_flag, p.status, 1)) goto done;
                     const uint32_t bar = full_lead + 8 * s, a_dst = a_smem + s * Cfg::A_STAGE, b_dst = b_smem + s * Cfg::B_STAGE;
                     if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
@@ -574,14 +611,14 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
                 if (!warp_wait(bar_tempty + 8 * buf, ((lt / NBUF) & 1) ^ 1, abort_flag, p.status, 2)) goto done;
                 tc_fence_after();
                 const uint32_t d = tmem_base + buf * BN;
-                for (int kt = 0; kt < p.k_tiles; kt++) {
+                for (int kt = k0; kt < k1; kt++) {
                     if (!warp_wait(bar_full + 8 * s, ph, abort_flag, p.status, 3)) goto done;
                     tc_fence_after();
                     if (elected) {
 #pragma unroll
                         for (int k = 0; k < KCH / 32; k++) {
-                            if (CG == 2) tc_mma_i8_pair_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)(kt | k));
-                            else tc_mma_i8_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)(kt | k));
+                            if (CG == 2) tc_mma_i8_pair_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)((kt - k0) | k));
+                            else tc_mma_i8_lh(d, a_lo + 2 * k, a_hi, b_lo + 2 * k, b_hi, IDESC, (uint32_t)((kt - k0) | k));
                         }
                         if (CG == 2) tc_commit_pair(bar_empty + 8 * s); else tc_commit(bar_empty + 8 * s);
                     }
@@ -667,10 +704,22 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
             const int place0 = now.m0 + (int)rank * BM + q * 32, rows_here = min(32, now.last - place0);
             if (!warp_wait(bar_tfull + 8 * buf, (lt / NBUF) & 1, abort_flag, p.status, 4)) goto done;
             tc_fence_after();
+            if (CS > 1) {  // the only tile
+                share_rs = rs;
+                if (part / OWN != share) {
+                    uint32_t v[32];
+                    tmem_ld_32(tmem_base + ((uint32_t)(q * 32) << 16) + part * 32, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const uint32_t dst = mapa_shared(sums_at(part, q, share), (uint32_t)(part / OWN));
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 512), "r"(v[4 * j]), "r"(v[4 * j + 1]), "r"(v[4 * j + 2]), "r"(v[4 * j + 3]) : "memory");
+                }
+                continue;
+            }
             if (t + units < tiles) fetch(t + units);
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + part * HN;
             const int n0 = now.n * BN + part * HN, size = p.dtype == TNNS_F32 ? 4 : 2;
-            const long long step = p.y_stride * size;
 #pragma unroll 1
             for (int i = 0; i < NC; i++) {
                 uint32_t v[32];
@@ -684,23 +733,7 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
                     }
                 }
                 if (i == 0) rs = row >= 0 ? p.scale[row] : 0.f;  // the next tile's
-                const int have = (p.N - n0 - 32 * i) * size;
-                if (rows_here > 0 && have > 0) {
-                    uint32_t w[16];
-                    const int x = (n0 + 32 * i) * size;
-                    unsigned char* base = reinterpret_cast<unsigned char*>(p.y);
-                    if (size == 4) {
-                        finish_words<16>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
-                        store_rows(w, stage, &maps.y, base, x, place0, step, rows_here, min(have, 64), p.y_vec, 4, lane);
-                        if (have > 64) {
-                            finish_words<16>(p.dtype, v + 16, rs_now, wsc + 32 * i + 16, p.alpha, mode, w);
-                            store_rows(w, stage, &maps.y, base, x + 64, place0, step, rows_here, min(have - 64, 64), p.y_vec, 4, lane);
-                        }
-                    } else {
-                        finish_words<32>(p.dtype, v, rs_now, wsc + 32 * i, p.alpha, mode, w);
-                        store_rows(w, stage, &maps.y, base, x, place0, step, rows_here, min(have, 64), p.y_vec, 2, lane);
-                    }
-                }
+                store_chunk(p, maps, v, rs_now, wsc + 32 * i, mode, stage, n0 + 32 * i, place0, rows_here, size, lane);
                 __syncwarp();
             }
         }
@@ -708,11 +741,40 @@ __global__ void __launch_bounds__(TcI8<BN, CG, GATHER>::THREADS, 1) gemm_i8_tc_k
 
 done:
     __syncwarp();
-    if (warp >= Cfg::EPI0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // results still on their way out of shared memory
     if (*abort_flag && warp == WARP_TMA && lane == 0) {
         // a wait gave up: give the copies already requested time to land before shared memory is released
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }
+    if (CS > 1) {
+        __syncwarp();
+        tc_fence_before();
+        cluster_sync_all();
+        tc_fence_after();
+        const int q = warp & 3, chunk = (warp - Cfg::EPI0) >> 2;
+        if (warp >= Cfg::EPI0 && chunk / OWN == share && unit < tiles && !*abort_flag) {
+            uint32_t v[32];
+            tmem_ld_32(tmem_base + ((uint32_t)(q * 32) << 16) + chunk * 32, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll 1
+            for (int i = 1; i < CS; i++) {
+                const uint32_t src = sums_at(chunk, q, (share + i) % CS);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    uint32_t x[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(src + j * 512) : "memory");
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[4 * j + k] += x[k];
+                }
+            }
+            __syncwarp();  // the sums are read: their place is the buffer for results
+            const Tile c = tile_at(unit);
+            const int n0 = c.n * BN + chunk * 32, place0 = c.m0 + q * 32, rows_here = min(32, c.last - place0), size = p.dtype == TNNS_F32 ? 4 : 2;
+            const int mode = p.alpha == 1.0f ? 0 : p.alpha > 0.0f && p.alpha < 1.0f ? 1 : 2;
+            store_chunk(p, maps, v, share_rs, s_ws + (warp - Cfg::EPI0) * 32, mode, s_stage + ((chunk % OWN) * 4 + q) * (CS - 1) * 1024, n0, place0, rows_here, size, lane);
+        }
+        __syncwarp();
+    }
+    if (warp >= Cfg::EPI0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // results still on their way out of shared memory
     tc_fence_before();
     if (CG == 2) cluster_sync_all(); else __syncthreads();
     if (warp == WARP_MMA) {
@@ -747,9 +809,9 @@ int launch(void (*kern)(Args...), tnns_cuda_ctx* ctx, int grid, int threads, siz
     return TNNS_OK;
 }
 
-template <int BN, int CG, bool GATHER>
+template <int BN, int CG, bool GATHER, int CS = 1>
 int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
-    using Cfg = TcI8<BN, CG, GATHER>;
+    using Cfg = TcI8<BN, CG, GATHER, CS>;
     MapsI8 maps = {};
     int rc = tnns_tensor_map_2d(&maps.q, 1, a.q, (unsigned long long)a.K, (unsigned long long)a.q_rows, (unsigned long long)a.q_stride, KCH, a.q_box, 128);
     if (rc) return rc;
@@ -760,7 +822,7 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
         const int size = tnns_dtype_bytes(a.dtype);
         if ((rc = tnns_tensor_map_2d(&maps.y, 1, a.y, (unsigned long long)a.N * size, (unsigned long long)a.places, (unsigned long long)a.y_stride * size, 64, 32, 64))) return rc;
     }
-    auto kern = gemm_i8_tc_kernel<BN, CG, GATHER>;
+    auto kern = gemm_i8_tc_kernel<BN, CG, GATHER, CS>;
     static bool smem_set[64] = {false};  // the attribute belongs to (function, device)
     if (!smem_set[ctx->device & 63]) {
         TNNS_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::smem(MAX_EXPERTS)));
@@ -769,8 +831,9 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     const long long n_blocks = (a.N + BN - 1) / BN;
     const long long most = ((long long)a.places + CG * BM - 1) / (CG * BM) + (a.offsets ? std::min(a.experts, a.places) : 0);
     if (most * n_blocks >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many tiles: %d places of %d channels", a.places, a.N);
-    const int grid = CG * (int)std::min<long long>(most * n_blocks, ctx->sm_count / CG);
-    return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG, stream, a, maps);
+    // shares (CS > 1): a cluster for every tile
+    const int grid = CG * CS * (int)(CS > 1 ? most * n_blocks : std::min<long long>(most * n_blocks, ctx->sm_count / CG));
+    return launch<GemmI8Args, MapsI8>(kern, ctx, grid, Cfg::THREADS, Cfg::smem(a.experts), CG * CS, stream, a, maps);
 }
 
 // Warps that share the K tiles: at least four tiles a warp, so that their loads overlap, unless the pieces do not fill the SMs.
@@ -810,12 +873,13 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     const cudaStream_t st = (cudaStream_t)stream;
     // places an expert has on average, experts that may have one, pieces of 64 channels of those
     const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);
-    const long long pieces = met * ((w->N + 63) / 64);
-    // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, tensor cores 14.9 / 10.8), or as many as make no more
-    // than a piece of 64 channels for every SM (1024 -> 1000, 64 / 128 rows: 3.4 / 5.5 us, tensor cores 6.6 / 6.7).  Experts: up to 32
+    const long long pieces = met * ((w->N + 63) / 64), sixteens = (rows + 15) / 16 * pieces;
+    // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, 33 on the tensor cores 9.7), or where pieces of 64 channels x
+    // 16 rows are no more than SMs and short enough together, the more of them the shorter (few rows' kernel / tensor cores: 128 x 1024 -> 1024
+    // 5.5 / 6.5 us, 128 x 2048 6.3 / 7.0, 128 x 4096 9.4 / 8.5; 64 x 8192 -> 1024 8.5 / 10.1, 64 x 16384 14.2 / 13.8).  Experts: up to 32
     // rows each, where those that have a row make fewer pieces than SMs (one token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two
     // tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8 experts, 1561 -> 226: 27 / 10.6).
-    const bool few = !d_offsets ? rows <= 32 || (rows + 15) / 16 * pieces <= ctx->sm_count : pieces < ctx->sm_count && rows <= 32;
+    const bool few = !d_offsets ? rows <= 32 || (sixteens <= ctx->sm_count && (10 * sixteens - 3 * ctx->sm_count) * w->k_tiles <= 100 * ctx->sm_count) : pieces < ctx->sm_count && rows <= 32;
     if (q_rows == 0 || few) return rows <= 8 ? launch_few<1>(ctx, a, st) : launch_few<2>(ctx, a, st);
     // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
     // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).
@@ -823,10 +887,27 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     // Tiles of 256 x 256 on block pairs, of 128 x 128 or of 128 x 64 on single blocks: what takes the fewest clocks, by the waves that the
     // launch's tiles make and the clocks of a K tile in each (measured with every SM at work: about 620, 530 and 410; the large tiles
     // are bound by the shared memory's bandwidth, the small ones by L2's).  1024 x 4096 -> 4096: pairs 17.6 us, 128 x 128 21.5; 512 rows 128 x
-    // 128 13.3, 128 x 64 18.6; 1024 x 4096 -> 1024: 128 x 64 11.3, 128 x 128 13.4.
+    // 128 13.3, 128 x 64 18.6; 1024 x 4096 -> 1024, sums not shared: 128 x 64 11.3, 128 x 128 13.4.
     const long long each = d_offsets ? met : 1;
-    auto clocks = [&](int tm, int tn, int units, int per_stage) { return ((rows + tm - 1) / tm * each * ((w->N + tn - 1) / tn) + units - 1) / units * per_stage; };
+    auto tiles = [&](int tm, int tn) { return (rows + tm - 1) / tm * each * ((w->N + tn - 1) / tn); };
+    auto clocks = [&](int tm, int tn, int units, int per_stage) { return (tiles(tm, tn) + units - 1) / units * per_stage * w->k_tiles; };
     const long long pair = clocks(256, 256, ctx->sm_count / 2, 620), wide = clocks(128, 128, ctx->sm_count, 530), narrow = clocks(128, 64, ctx->sm_count, 410);
+    // Fewer tiles than SMs: clusters that share them, where their shorter sums save more than the exchange takes (about 5000 clocks among
+    // four, 4400 between two; alone / shared: 256 x 4096 -> 1024 11.1 / 8.7 us, 282 x 14050 -> 1529 31.0 / 19.5, 1024 x 4096 -> 1024 11.2 / 10.2, but 128 x
+    // 1024 -> 4096 6.3 / 8.0).  Clusters of four do not find room on every SM.
+    if (!d_offsets) {
+        const long long best = std::min(std::min(pair, wide), narrow);
+        auto shared = [&](int tn, int cs, int units, int per_stage, int exchange) {
+            return tiles(BM, tn) <= units && w->k_tiles >= cs ? (long long)(w->k_tiles + cs - 1) / cs * per_stage + exchange : best;
+        };
+        const long long quarters = shared(128, 4, ctx->sm_count / 4 - 4, 530, 5000), halves = shared(128, 2, ctx->sm_count / 2, 530, 4400), narrow_halves = shared(64, 2, ctx->sm_count / 2, 410, 4400);
+        const long long least = std::min(std::min(quarters, halves), narrow_halves);
+        if (least < best) {
+            if (quarters == least) return launch_tc<128, 1, false, 4>(ctx, a, st);
+            if (halves == least) return launch_tc<128, 1, false, 2>(ctx, a, st);
+            return launch_tc<64, 1, false, 2>(ctx, a, st);
+        }
+    }
     if (pair <= wide && pair <= narrow) return d_rows ? launch_tc<256, 2, true>(ctx, a, st) : launch_tc<256, 2, false>(ctx, a, st);
     if (wide <= narrow) return d_rows ? launch_tc<128, 1, true>(ctx, a, st) : launch_tc<128, 1, false>(ctx, a, st);
     return d_rows ? launch_tc<64, 1, true>(ctx, a, st) : launch_tc<64, 1, false>(ctx, a, st);

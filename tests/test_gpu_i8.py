@@ -172,6 +172,59 @@ def test_gemm_strides(M, K, N, q_stride, y_stride, shift, dtype, gpu_ctx):
     assert (np.abs(y - want) <= product_error(want, dtype)).all()
 
 
+# Fewer tiles than the GPU has SMs and long sums: blocks that share a tile's sum.
+FEW_TILES = [
+    (128, 4096, 4096, 4096, 0), (33, 2048, 4096, 4104, 8), (65, 4096, 2500, 2501, 1), (100, 2500, 2333, 2333, 0), (1, 131071, 4224, 4224, 0), (100, 131071, 300, 301, 3),
+    (256, 4096, 4096, 4096, 0), (282, 14050, 1529, 1529, 0), (1030, 5000, 901, 904, 0), (1500, 3333, 231, 231, 1), (2738, 8443, 130, 132, 2), (640, 2100, 700, 704, 0),
+    (500, 1024, 1000, 1000, 0), (320, 6000, 1536, 1600, 16), (257, 513, 1111, 1111, 0), (4000, 1030, 40, 41, 0)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("M,K,N,y_stride,shift", FEW_TILES, ids=str)
+def test_gemm_few_tiles(M, K, N, y_stride, shift, dtype, gpu_ctx):
+    g = gen(M + 3 * K + 5 * N)
+    q, w = int8(g, M, K), int8(g, N, K)
+    scale, w_scale = torch.rand(M, generator=g) * 0.01, torch.rand(N, generator=g) * 0.001
+    alpha = [1.0, 0.5, -0.25][(M + K + N) % 3]
+    y = run_gemm(gpu_ctx, q, scale, w, w_scale, dtype, alpha, y_stride=y_stride, shift=shift)
+    want = product(q.numpy(), scale.numpy(), w.numpy(), w_scale.numpy(), alpha)
+    assert (np.abs(y - want) <= product_error(want, dtype)).all()
+
+
+def test_gemm_few_tiles_in_a_row(gpu_ctx):
+    """Products whose blocks share sums, each reading what the one in front wrote, in one captured graph replayed: no run differs."""
+    g = gen(77)
+    M, D, H = 128, 4096, 2048
+    s1, s2 = torch.rand(D, generator=g) * 1e-4, torch.rand(H, generator=g) * 1e-4
+    up, down = (gpu_ctx.upload_weights_i8(int8(g, n, k).data_ptr(), s.data_ptr(), n, k) for n, k, s in ((H, D, s2), (D, H, s1)))
+    x0 = torch.randn(M, D, generator=g).cuda()
+    x, y = x0.clone(), torch.empty(M, H, device="cuda")
+    qx, qy = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, H, dtype=torch.int8, device="cuda")
+    sx, sy = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+
+    def run():
+        for _ in range(6):
+            gpu_ctx.quantise_i8(x.data_ptr(), ft.F32, qx.data_ptr(), sx.data_ptr(), M, D, stream=stream())
+            gpu_ctx.gemm_i8(up, qx.data_ptr(), sx.data_ptr(), y.data_ptr(), ft.F32, M, 0.5, stream=stream())
+            gpu_ctx.quantise_i8(y.data_ptr(), ft.F32, qy.data_ptr(), sy.data_ptr(), M, H, stream=stream())
+            gpu_ctx.gemm_i8(down, qy.data_ptr(), sy.data_ptr(), x.data_ptr(), ft.F32, M, 1.0, stream=stream())
+
+    run()
+    gpu_ctx.sync()
+    want = x.clone()
+    assert bool(torch.isfinite(want).all()) and bool(want.any())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(20):
+        x.copy_(x0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+    up.free()
+    down.free()
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_gemm_largest_sums(M, gpu_ctx):
     """The longest rows of the largest products: the sum is a few products short of 2^31."""

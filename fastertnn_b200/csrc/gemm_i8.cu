@@ -874,12 +874,14 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     // places an expert has on average, experts that may have one, pieces of 64 channels of those
     const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);
     const long long pieces = met * ((w->N + 63) / 64), sixteens = (rows + 15) / 16 * pieces;
-    // Few rows.  One kernel: up to 32 rows (4096 -> 4096, 16 / 32 rows: 6.3 / 10.1 us, 33 on the tensor cores 9.7), or where pieces of 64 channels x
-    // 16 rows are no more than SMs and short enough together, the more of them the shorter (few rows' kernel / tensor cores: 128 x 1024 -> 1024
-    // 5.5 / 6.5 us, 128 x 2048 6.3 / 7.0, 128 x 4096 9.4 / 8.5; 64 x 8192 -> 1024 8.5 / 10.1, 64 x 16384 14.2 / 13.8).  Experts: up to 32
-    // rows each, where those that have a row make fewer pieces than SMs (one token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two
-    // tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8 experts, 1561 -> 226: 27 / 10.6).
-    const bool few = !d_offsets ? rows <= 32 || (sixteens <= ctx->sm_count && (10 * sixteens - 3 * ctx->sm_count) * w->k_tiles <= 100 * ctx->sm_count) : pieces < ctx->sm_count && rows <= 32;
+    // Few rows.  One kernel: up to 8 rows; up to 32, or where pieces of 64 channels x 16 rows are no more than SMs, if the pieces' sums are
+    // short enough, the more pieces the shorter (few rows' kernel / tensor cores: 16 rows, 4096 -> 4096 6.3 / 10.0 us, 4096 -> 8192 10.6 / 11.5, 8192 ->
+    // 8192 18.1 / 16.5; 24 rows 9.4 / 10.4, 16.6 / 12.4, 28.3 / 16.7; 128 x 1024 -> 1024 5.5 / 6.5, 128 x 2048 6.3 / 7.0, 128 x 4096 9.4 / 8.5; 64 x 8192
+    // -> 1024 8.5 / 10.1, 64 x 16384 14.2 / 13.8).  Experts: up to 32 rows each, where those that have a row make fewer pieces than SMs (one
+    // token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8
+    // experts, 1561 -> 226: 27 / 10.6).
+    const bool short_sums = (10 * sixteens - 3 * ctx->sm_count) * w->k_tiles <= (rows <= 32 ? 200LL : 100LL) * ctx->sm_count;
+    const bool few = !d_offsets ? rows <= 8 || (short_sums && (rows <= 32 || sixteens <= ctx->sm_count)) : pieces < ctx->sm_count && rows <= 32;
     if (q_rows == 0 || few) return rows <= 8 ? launch_few<1>(ctx, a, st) : launch_few<2>(ctx, a, st);
     // Rows of q by boxes of 32 or 64 where most tiles hold no more (8 tokens, 8 of 64 experts: 22.2 / 21.1 us; two boxes instead of a whole
     // one cost 64 x 4096 -> 4096 11.0 / 14.4 us).

@@ -176,7 +176,8 @@ def test_gemm_strides(M, K, N, q_stride, y_stride, shift, dtype, gpu_ctx):
 FEW_TILES = [
     (128, 4096, 4096, 4096, 0), (33, 2048, 4096, 4104, 8), (65, 4096, 2500, 2501, 1), (100, 2500, 2333, 2333, 0), (1, 131071, 4224, 4224, 0), (100, 131071, 300, 301, 3),
     (256, 4096, 4096, 4096, 0), (282, 14050, 1529, 1529, 0), (1030, 5000, 901, 904, 0), (1500, 3333, 231, 231, 1), (2738, 8443, 130, 132, 2), (640, 2100, 700, 704, 0),
-    (500, 1024, 1000, 1000, 0), (320, 6000, 1536, 1600, 16), (257, 513, 1111, 1111, 0), (4000, 1030, 40, 41, 0)]
+    (500, 1024, 1000, 1000, 0), (320, 6000, 1536, 1600, 16), (257, 513, 1111, 1111, 0), (4000, 1030, 40, 41, 0),
+    (9, 8200, 8190, 8190, 1), (20, 4100, 8200, 8208, 0), (32, 2050, 9001, 9001, 1)]
 
 
 @pytest.mark.parametrize("dtype", DT)

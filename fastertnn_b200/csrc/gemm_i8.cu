@@ -140,9 +140,8 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 // instruction), so a load takes eight whole lines, four instructions multiply a K tile of 2 KB, and no byte passes through shared
 // memory.  The order of K within the tile is the same for weights and rows.  1 x 4096 -> 4096: 5.0 us = 3.4 TB/s, of which the launch and
 // the first bytes' way take 2.4.
-template <int NT>
+template <int NT, int U>  // U: K tiles whose loads a warp issues together
 __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int log_s) {
-    constexpr int U = NT == 1 ? 4 : 2;  // K tiles whose loads a warp issues together
     extern __shared__ int2 s_range[];
     int* s_first = reinterpret_cast<int*>(s_range + p.experts);
     __shared__ int s_sum[FEW_WARPS][NT][16 * 8];
@@ -847,7 +846,12 @@ int launch_few(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     const long long items = high * ((a.N + wide - 1) / wide);
     if (items >= 0x3FFFFFFFLL) return tnns_fail(TNNS_ERR_UNSUPPORTED, "too many pieces: %d places of %d channels", a.places, a.N);
     const int grid = (int)std::min<long long>(items, 2LL * ctx->sm_count);  // as many blocks as are resident
-    return launch<GemmI8Args, int>(gemm_i8_few_kernel<NT>, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, log_s);
+    // As many tiles' loads at once as a warp has tiles, four at most (always four / as many: 1 x 1024 -> 1000 3.45 / 2.3 us, 1 x 1024 -> 8192 7.0 /
+    // 4.2, 16 x 1024 -> 8192, always two / one, 5.9 / 5.0); experts' few pieces take two (one token, 8 of 64, 4096 -> 1024: four 9.5 / two 7.9).
+    const int deep = (a.k_tiles + (1 << log_s) - 1) >> log_s;
+    auto go = [&](void (*kern)(GemmI8Args, int)) { return launch<GemmI8Args, int>(kern, ctx, grid, FEW_WARPS * 32, list_bytes(a.experts), 1, stream, a, log_s); };
+    if (deep == 1) return go(gemm_i8_few_kernel<NT, 1>);
+    return NT == 2 || deep == 2 || a.offsets ? go(gemm_i8_few_kernel<NT, 2>) : go(gemm_i8_few_kernel<1, 4>);
 }
 
 int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t* d_q, long long q_stride, const float* d_scale, int q_rows,
@@ -878,7 +882,7 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     // short enough, the more pieces the shorter (few rows' kernel / tensor cores: 16 rows, 4096 -> 4096 6.3 / 10.0 us, 4096 -> 8192 10.6 / 11.5, 8192 ->
     // 8192 18.1 / 16.5; 24 rows 9.4 / 10.4, 16.6 / 12.4, 28.3 / 16.7; 128 x 1024 -> 1024 5.5 / 6.5, 128 x 2048 6.3 / 7.0, 128 x 4096 9.4 / 8.5; 64 x 8192
     // -> 1024 8.5 / 10.1, 64 x 16384 14.2 / 13.8).  Experts: up to 32 rows each, where those that have a row make fewer pieces than SMs (one
-    // token, 8 of 64 experts, 2048 -> 1024: 8.0 us, tensor cores 9.2; two tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8
+    // token, 8 of 64 experts, 2048 -> 1024: 6.0 us, tensor cores 9.2; two tokens 10.8 / 9.9; eight, 1024 -> 2048: 24.8 / 20.5; 352 rows each, 8
     // experts, 1561 -> 226: 27 / 10.6).
     const bool short_sums = (10 * sixteens - 3 * ctx->sm_count) * w->k_tiles <= (rows <= 32 ? 200LL : 100LL) * ctx->sm_count;
     const bool few = !d_offsets ? rows <= 8 || (short_sums && (rows <= 32 || sixteens <= ctx->sm_count)) : pieces < ctx->sm_count && rows <= 32;

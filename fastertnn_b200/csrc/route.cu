@@ -324,13 +324,16 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
             if (__any_sync(FULL, third)) certain = false;
             else kept = groups_exact<T>(p, row, lane, key[0] == -INFINITY ? MAX_E : at.e0 + register_of(key[0]), key[1] == -INFINITY ? MAX_E : at.e0 + register_of(key[1]), c.top);
         }
-        if (!kept) key[0] = -INFINITY;
+        // every key of the lane, not its first alone: what is taken moves the next one up
+#pragma unroll
+        for (int r = 0; r < NPL; r++) key[r] = kept ? key[r] : -INFINITY;
     }
     // lane j < n: the j-th best key and its expert
     float mine_key = -INFINITY;
     int mine = MAX_E, n = p.top_k, first = at.e0 + register_of(key[0]);
     auto pop = [&](int j) {
         const float m = warp_max(key[0]);
+        if (m == -INFINITY) return false;  // no expert is left
         const int e = (int)__reduce_min_sync(FULL, key[0] == m ? (unsigned)first : (unsigned)MAX_E);
         if (lane == j) {
             mine_key = m;
@@ -342,8 +345,9 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
             key[NPL - 1] = -INFINITY;
             first = at.e0 + register_of(key[0]);
         }
+        return true;
     };
-    for (int j = 0; j < n; j++) pop(j);
+    for (int j = 0; j < n && pop(j);) j++;
     // those behind the last slot that are near it, and near each other, are candidates too
     float last = __shfl_sync(FULL, mine_key, n - 1);
     for (;;) {

@@ -1,0 +1,54 @@
+"""GPU suite: routing limited to groups, where groups run out of experts and where their worths are hard to compare in fp32."""
+import numpy as np
+import pytest
+import torch
+
+import fastertnn_b200 as ft
+from i8_reference import DT, route
+from test_gpu_route import INF, NAN, check, gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("masked_by", ["logits", "bias", "both"])
+@pytest.mark.parametrize("E,k,groups,top_groups", [
+    (64, 8, 8, 1), (64, 8, 8, 4), (32, 4, 16, 4), (256, 8, 8, 4), (128, 8, 4, 2), (160, 6, 8, 3), (384, 8, 8, 2), (96, 8, 3, 1), (1024, 32, 32, 4), (1024, 16, 2, 1),
+    (1020, 10, 17, 3), (320, 32, 5, 2)], ids=str)
+def test_kept_groups_run_out_of_experts(E, k, groups, top_groups, masked_by, group_top, score, gpu_ctx):
+    """The best groups hold fewer experts than slots, the others (the first group among them) hold many: none of theirs is chosen."""
+    g, T, size = gen(E + k + groups), 60, E // groups
+    logits = torch.randn(T, E, generator=g) * 0.5 - 3
+    best = torch.arange(groups) >= groups - top_groups if masked_by == "bias" else None  # (a bias is the same for all tokens)
+    bias = torch.randn(E, generator=g) * 0.01 if masked_by != "logits" else None
+    for t in range(T):
+        chosen = torch.arange(groups)[best] if best is not None else 1 + torch.randperm(groups - 1, generator=g)[:top_groups] if groups > top_groups else torch.arange(groups)
+        for i in chosen.tolist():
+            there = torch.randperm(size, generator=g)[:t % 4]
+            if masked_by == "bias":
+                logits[t, i * size:(i + 1) * size] += 6
+            else:
+                keep = logits[t, i * size + there] + 6
+                logits[t, i * size:(i + 1) * size] = [-INF, NAN][t % 2]
+                logits[t, i * size + there] = keep
+    if masked_by == "bias":
+        for i in torch.arange(groups)[best].tolist():
+            bias[i * size:(i + 1) * size] = [-INF, NAN][i % 2]
+            bias[i * size + torch.randperm(size, generator=g)[:i % 3]] = 0.25
+    r = ft.Route(E, k, score, groups, top_groups, group_top, 1, 2.5)
+    check(gpu_ctx, r, logits, bias)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_one_expert_left_in_every_kept_group(with_bias, dtype, gpu_ctx):
+    """Four kept groups with an expert each, four whole ones that are not kept: four slots stay empty."""
+    logits = torch.randn(1, 256, generator=gen(1)) * 0.1
+    logits[0, 128:] = -INF
+    for e, v in ((130, 5.0), (165, 6.0), (200, 7.0), (230, 8.0)):
+        logits[0, e] = v
+    r = ft.Route(256, 8, 0, 8, 4, 1, 1, 1.0)
+    logits, bias = logits.to(DT[dtype]), torch.zeros(256) if with_bias else None
+    assert route(logits, bias, r)[0].tolist() == [[230, 200, 165, 130, -1, -1, -1, -1]]
+    check(gpu_ctx, r, logits, bias)

@@ -103,7 +103,8 @@ __device__ __forceinline__ double score_of(const RouteArgs& p, double l, double 
     return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / all;
 }
 // The two best values of a group, (a, b) being those of its lanes, and whether the group is among the best: groups ranked by a, or by
-// a + b.  Returns the group's worth.
+// a + b.  Returns the group's worth: -inf where it has no expert, and there alone (a sum of two finite values that leaves fp32 counts as
+// the outermost finite float; in 64 bits none leaves).
 template <typename Key>
 __device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, Key a, Key b, bool& kept) {
     for (int d = 1; d < at.L; d <<= 1) {
@@ -111,7 +112,9 @@ __device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, K
         b = fmax(fmin(a, oa), fmax(b, ob));
         a = fmax(a, oa);
     }
-    const Key none = -INFINITY, worth = p.group_top == 2 && b != none ? a + b : a;
+    const Key none = -INFINITY;
+    Key worth = p.group_top == 2 && b != none ? a + b : a;
+    if (sizeof(Key) == 4 && a != none) worth = fmin(fmax(worth, (Key)-3.402823466e38f), (Key)3.402823466e38f);
     int better = 0;
     for (int g = 0; g < p.groups; g++) {
         const Key o = __shfl_sync(FULL, worth, g << (5 - p.glog));

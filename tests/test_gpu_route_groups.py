@@ -52,3 +52,32 @@ def test_one_expert_left_in_every_kept_group(with_bias, dtype, gpu_ctx):
     logits, bias = logits.to(DT[dtype]), torch.zeros(256) if with_bias else None
     assert route(logits, bias, r)[0].tolist() == [[230, 200, 165, 130, -1, -1, -1, -1]]
     check(gpu_ctx, r, logits, bias)
+
+
+LOWEST, LARGEST = -float(np.finfo(np.float32).max), float(np.finfo(np.float32).max)
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("values", [[LOWEST], [LOWEST, 0.1], [LOWEST, -2e38, -1.8e38, 0.0], [LARGEST, 2e38, LOWEST], [INF, LARGEST, 0.0, -2e38]], ids=str)
+@pytest.mark.parametrize("E,k,groups,top_groups", [(12, 6, 3, 2), (64, 16, 8, 2), (128, 16, 4, 2), (256, 8, 8, 4), (1024, 32, 16, 3)], ids=str)
+def test_biases_whose_sums_leave_fp32(E, k, groups, top_groups, values, group_top, score, gpu_ctx):
+    """Two biases of a group that add up to more (or less) than the largest float: such a group still has experts, and its place."""
+    g, T, size = gen(E + len(values)), 80, E // groups
+    bias = torch.tensor(values)[torch.randint(0, len(values), (E,), generator=g)]
+    for i in range(0, groups, 2):  # groups all alike
+        bias[i * size:(i + 1) * size] = values[i // 2 % len(values)]
+    logits = torch.randn(T, E, generator=g)
+    for t in range(1, T):  # groups without experts, in front of those and between them
+        for i in torch.randperm(groups, generator=g)[:t % groups].tolist():
+            logits[t, i * size:(i + 1) * size] = -INF
+    check(gpu_ctx, ft.Route(E, k, score, groups, top_groups, group_top, 1, 1.0), logits, bias)
+
+
+def test_lowest_biases_beside_a_group_without_experts(gpu_ctx):
+    """Group 0 has no expert, group 1 the type's lowest value as its mask, group 2 ordinary biases: 2 and 1 are kept."""
+    logits, bias = torch.zeros(1, 12), torch.zeros(12)
+    logits[0, :4], bias[4:8] = -INF, LOWEST
+    r = ft.Route(12, 6, 1, 3, 2, 2, 1, 1.0)
+    assert route(logits, bias, r)[0].tolist() == [[8, 9, 10, 11, 4, 5]]
+    check(gpu_ctx, r, logits, bias)

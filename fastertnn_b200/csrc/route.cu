@@ -102,11 +102,11 @@ __device__ __forceinline__ float score_of(const RouteArgs& p, float l, float top
 __device__ __forceinline__ double score_of(const RouteArgs& p, double l, double top, double all) {
     return p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / all;
 }
-// The two best values of a group, (a, b) being those of its lanes, and whether the group is among the best: groups ranked by a, or by
+// (a, b): the two best values of the lane, on return those of its group; kept: whether the group is among the best, ranked by a, or by
 // a + b.  Returns the group's worth: -inf where it has no expert, and there alone (a sum of two finite values that leaves fp32 counts as
 // the outermost finite float; in 64 bits none leaves).
 template <typename Key>
-__device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, Key a, Key b, bool& kept) {
+__device__ __forceinline__ Key rank_group(const RouteArgs& p, const Lanes& at, Key& a, Key& b, bool& kept) {
     for (int d = 1; d < at.L; d <<= 1) {
         const Key oa = __shfl_xor_sync(FULL, a, d), ob = __shfl_xor_sync(FULL, b, d);
         b = fmax(fmin(a, oa), fmax(b, ob));
@@ -235,7 +235,8 @@ __device__ __noinline__ bool groups_exact(const RouteArgs& p, const T* row, int 
     }
     __syncwarp();
     bool kept;
-    rank_group<double>(p, at, fmax(v[0], v[1]), fmin(v[0], v[1]), kept);
+    double a = fmax(v[0], v[1]), b = fmin(v[0], v[1]);
+    rank_group<double>(p, at, a, b, kept);
     return kept;
 }
 
@@ -316,12 +317,15 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
         }
         bool kept;
         const float worth = rank_group<float>(p, at, a, b, kept);
-        // the worst group that is kept against the best that is not
-        const float best_out = warp_max(kept || at.group >= p.groups ? -INFINITY : worth), worst_in = -warp_max(kept ? -worth : -INFINITY);
-        // (a score made of a logit that lost LOG bits is off by |logit| times that; s * |logit| <= s * |top| + 1 / e)
-        const float lost = sums ? (1.0f + (p.sigmoid ? 0.f : fabsf(c.top) * fabsf(worst_in))) * tol1 : 0.f;
-        const float tol = 2 * ((NPL + 24) * 0x1p-23f * (p.bias || sums) + fmaxf(fabsf(worst_in), fabsf(best_out)) * (tol1 + 0x1p-22f) + lost) + 1e-30f;  // (a worth is made of two)
-        if (!(best_out == -INFINITY || worst_in - best_out > tol)) {
+        // A worth is off by what its parts are: each keeps the errors of a score, and |part| times those of its bits (their sum may be far
+        // smaller than they are).  A score made of a logit that lost LOG bits is off by |logit| times that; s * |logit| <= s * |top| + 1 / e.
+        const bool there = a != -INFINITY;
+        const float parts = fabsf(a) + (p.group_top == 2 && b != -INFINITY ? fabsf(b) : 0.f);
+        const float lost = sums ? (1.0f + (p.sigmoid ? 0.f : fabsf(c.top) * worth)) * tol1 : 0.f;
+        const float off = (NPL + 24) * 0x1p-23f * (p.bias || sums) + parts * (tol1 + 0x1p-22f) + lost + 1e-30f;
+        // the least that a kept group can be worth against the most that one can that is not
+        const float best_out = warp_max(there && !kept ? worth + off : -INFINITY), worst_in = -warp_max(there && kept ? off - worth : -INFINITY);
+        if (!(best_out == -INFINITY || worst_in > best_out)) {
             // the lanes' two best are certain as such unless a third is near them
             const bool third = NPL > 2 && key[1] != -INFINITY && key[NPL > 2 ? 2 : 1] != -INFINITY && near(key[1], key[NPL > 2 ? 2 : 1]);
             if (__any_sync(FULL, third)) certain = false;

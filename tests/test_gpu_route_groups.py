@@ -81,3 +81,17 @@ def test_lowest_biases_beside_a_group_without_experts(gpu_ctx):
     r = ft.Route(12, 6, 1, 3, 2, 2, 1, 1.0)
     assert route(logits, bias, r)[0].tolist() == [[8, 9, 10, 11, 4, 5]]
     check(gpu_ctx, r, logits, bias)
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("size_of_bias", [30.0, 1000.0, 1e6])
+@pytest.mark.parametrize("E,k,groups,top_groups", [(32, 4, 8, 3), (64, 8, 8, 2), (256, 8, 8, 4), (96, 8, 3, 1), (512, 16, 2, 1), (1024, 8, 32, 16)], ids=str)
+def test_worths_of_parts_that_cancel(E, k, groups, top_groups, size_of_bias, score, gpu_ctx):
+    """A group's two best are far above and far below zero, and their sum is not: groups are ranked by that sum as 64 bits have it."""
+    g, T, size = gen(E + groups), 100, E // groups
+    bias = torch.full((E,), -3 * size_of_bias)
+    for i in range(groups):
+        up, down = torch.randperm(size, generator=g)[:2].tolist()
+        bias[i * size + up], bias[i * size + down] = size_of_bias, -size_of_bias
+    logits = torch.randn(T, E, generator=g)
+    check(gpu_ctx, ft.Route(E, k, score, groups, top_groups, 2, 1, 1.0), logits, bias)

@@ -44,7 +44,9 @@ struct Lanes {
         have = group < p.groups ? min(max(p.group_size - in, 0), p.per) : 0;
     }
 };
-// Values first .. first + NPL - 1 of a row, those past `have` as -inf.  vec: four at a time (rows and `have` allow it).
+// Values first .. first + NPL - 1 of a row, those past `have` as -inf.  vec: four at a time (rows and `have` allow it).  Plain loads, here
+// and wherever these kernels read an input: the launch in front may still write it while the block is resident, so it is no read-only
+// data of the kernel.
 template <typename T, int NPL>
 __device__ __forceinline__ void load_values(const T* at, int have, bool vec, float (&v)[NPL]) {
     if (NPL >= 4 && vec) {
@@ -53,10 +55,10 @@ __device__ __forceinline__ void load_values(const T* at, int have, bool vec, flo
             v[r] = v[r + 1] = v[r + 2] = v[r + 3] = -INFINITY;
             if (r < have) {
                 if constexpr (sizeof(T) == 4) {
-                    const float4 f = __ldg(reinterpret_cast<const float4*>(at + r));
+                    const float4 f = *reinterpret_cast<const float4*>(at + r);
                     v[r] = f.x; v[r + 1] = f.y; v[r + 2] = f.z; v[r + 3] = f.w;
                 } else {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(at + r));
+                    const uint2 u = *reinterpret_cast<const uint2*>(at + r);
                     const unsigned short h[4] = {(unsigned short)u.x, (unsigned short)(u.x >> 16), (unsigned short)u.y, (unsigned short)(u.y >> 16)};
 #pragma unroll
                     for (int i = 0; i < 4; i++) v[r + i] = to_f32(*reinterpret_cast<const T*>(&h[i]));
@@ -156,7 +158,7 @@ __device__ __noinline__ int choose_exact(const RouteArgs& p, const T* row, int l
         if (v != none && (p.bias || (grouped && p.group_top == 2))) {
             v = score_of(p, v, top, all);
             if (p.bias) {
-                const float c = __ldg(p.bias + at.e0 + r);
+                const float c = p.bias[at.e0 + r];
                 key[r] = v = barred(c) ? none : v + (double)bounded(c);
             }
         }
@@ -230,7 +232,7 @@ __device__ __noinline__ bool groups_exact(const RouteArgs& p, const T* row, int 
         v[i] = -INFINITY;
         if (e < MAX_E) {
             const double l = (double)bounded(to_f32(row[e]));
-            v[i] = by_logit ? l : score_of(p, l, (double)top, all) + (p.bias ? (double)bounded(__ldg(p.bias + e)) : 0.0);
+            v[i] = by_logit ? l : score_of(p, l, (double)top, all) + (p.bias ? (double)bounded(p.bias[e]) : 0.0);
         }
     }
     __syncwarp();
@@ -371,7 +373,7 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
     float l = 0.f, b = 0.f;
     if (mine_key != -INFINITY && mine < p.E) {
         l = to_f32(row[mine]);
-        if (p.bias) b = __ldg(p.bias + mine);
+        if (p.bias) b = p.bias[mine];
     }
     const float prev_key = __shfl_up_sync(FULL, mine_key, 1), prev_l = __shfl_up_sync(FULL, l, 1), prev_b = __shfl_up_sync(FULL, b, 1);
     const int prev = __shfl_up_sync(FULL, mine, 1);

@@ -185,8 +185,10 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 // integers, NV chunks a thread: every element is read once.  LONG: rows that do not fit; the chunks past the kept ones are read a
 // second time.  The form for few rows (all latency) and for rows too long for the ring below.  (Groups that went on to another row and
 // requested it ahead were slower, 51 against 33 us for 8192 x 4096 bf16: their registers cost more rows in flight than that gave.)
+// The input may be what the launch in front is still writing: no __restrict__ on it and no __ldg in this file, which would promise that
+// it does not change while the kernel runs.
 template <typename T, int GROUP, int NV, bool MIS, bool LONG>
-__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(const T* __restrict__ x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(const T* x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
                                                                               float* __restrict__ scale, int M, int K) {
     constexpr int VE = Chunk<T>::VE, ROWS = GROUP < 256 ? 256 / GROUP : 1;
     __shared__ uint32_t s_top[32];
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
 // rows in registers 33) and short rows (20000 x 512 bf16: 12.4 us).
 constexpr int RING_WARPS = 12, RING_MAX_SLOTS = 8, RING_BYTES = 200 * 1024;
 template <typename T, bool MIS>
-__global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const T* __restrict__ x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
+__global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const T* x, long long x_stride, int8_t* __restrict__ q, long long q_stride,
                                                                          float* __restrict__ scale, int M, int K, int slots, int slot_bytes, unsigned int* status) {
     extern __shared__ __align__(16) unsigned char s_ring[];
     __shared__ uint64_t s_bar[RING_WARPS * RING_MAX_SLOTS];
@@ -415,8 +417,8 @@ __global__ void __launch_bounds__(256) combine_kernel(CombineArgs p) {
         float w[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            at[u] = j0 + u < p.top_k ? __ldg(slots + j0 + u) : -1;
-            w[u] = j0 + u < p.top_k ? __ldg(weights + j0 + u) : 0.f;
+            at[u] = j0 + u < p.top_k ? slots[j0 + u] : -1;
+            w[u] = j0 + u < p.top_k ? weights[j0 + u] : 0.f;
         }
         uint4 a[U], b[MIS ? U : 1];
 #pragma unroll

@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP) quantise_i8_kernel(
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long m = (long long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / GROUP : 0);
-    const int lane = threadIdx.x % GROUP, chunks = (K + VE - 1) / VE;
+    const int lane = threadIdx.x % GROUP, chunks = K / VE + (K % VE != 0);
     if (m >= M) return;  // (a whole group, and with several a whole warp)
     const T* row = x + m * x_stride;
     Chunk<T> c[NV];
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(RING_WARPS * 32, 1) quantise_ring_kernel(const
     __shared__ uint64_t s_bar[RING_WARPS * RING_MAX_SLOTS];
     __shared__ int s_abort;
     constexpr int VE = Chunk<T>::VE;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (K + VE - 1) / VE, whole = K / VE;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = K / VE + (K % VE != 0), whole = K / VE;
     const uint32_t bars = smem_u32(s_bar + warp * RING_MAX_SLOTS);
     unsigned char* ring = s_ring + (size_t)warp * slots * slot_bytes;
     if (threadIdx.x == 0) s_abort = 0;
@@ -320,7 +320,7 @@ int launch_rows(const T* x, long long x_stride, int8_t* q, long long q_stride, f
 // row in four chunks each; a few rows by themselves take more threads (the launch is all latency then).
 template <typename T, bool MIS>
 int launch_quantise(tnns_cuda_ctx* ctx, const T* x, long long x_stride, int8_t* q, long long q_stride, float* scale, int M, int K, cudaStream_t st) {
-    const int chunks = (K + Chunk<T>::VE - 1) / Chunk<T>::VE;
+    const int chunks = K / Chunk<T>::VE + (K % Chunk<T>::VE != 0);  // (K may be any int)
     const bool many = M > ctx->sm_count;
     const long long slot = (((long long)K * sizeof(T) + 15) / 16 + 1) * 16;  // a row may touch one 16-byte vector more than its size
     if (M >= 2LL * RING_WARPS * ctx->sm_count && slot * RING_WARPS <= RING_BYTES) {

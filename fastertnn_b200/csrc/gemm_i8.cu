@@ -48,7 +48,8 @@ struct GemmI8Args {
     void* y;
     long long y_stride;
     int q_rows, places, experts, N, K, n_tiles, k_tiles;
-    int dtype, y_vec;  // result type; bytes that may be stored at once everywhere in y
+    int dtype;
+    bool y_maps;       // results may leave as tensor copies: 16 bytes may be stored at once everywhere in y
     int q_box;         // rows of a tensor copy of q
     float alpha;
     unsigned int* status;
@@ -342,19 +343,19 @@ __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
 }
 // 64 bytes of each of a warp's rows to y: w = those of the lane's row; they leave through the warp's 32 x 64 bytes of shared memory,
 // the 16-byte pieces of a row in the pattern piece ^ (row / 2) % 4 (the copy engine's 64-byte swizzle, free of bank conflicts).
-// Whole blocks go out as one tensor copy where y allows it (vec >= 16: bytes that may be stored at once everywhere in y; a copy that
+// Whole blocks go out as one tensor copy where y allows it (maps: 16 bytes may be stored at once everywhere in y; a copy that
 // ends inside 16 bytes of a row would write all of them).  A store by lanes, each 32 bytes of its own row, took 32 bytes a clock off the
 // path that also feeds the tensor core: 65536 x 1024 -> 2048 bf16 in 134 us against 118, fp32 177 against 143.  The rest the warp writes
 // along the rows (4096 x 1024 -> 4097: 37 us, by lanes 190).  x, row0: first byte of the row, first row; have: bytes of a row that exist
 // (a multiple of `size`, an element's bytes); step: bytes from row to row.
 __device__ __forceinline__ void store_rows(const uint32_t (&w)[16], uint32_t* stage, const void* tmap, unsigned char* base, int x, int row0, long long step, int rows,
-                                           int have, int vec, int size, int lane) {
+                                           int have, bool maps, int size, int lane) {
     auto at = [&](int row, int word) { return stage + row * 16 + ((((word >> 2) ^ (row >> 1)) & 3) << 2) + (word & 3); };
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the copy before has read the buffer
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(at(lane, i)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    if (vec >= 16 && rows == 32 && have == 64) {
+    if (maps && rows == 32 && have == 64) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
@@ -441,20 +442,21 @@ __device__ __forceinline__ void store_chunk(const GemmI8Args& p, const MapsI8& m
     uint32_t w[16];
     if (size == 4) {
         finish_words<16>(p.dtype, v, rs, ws, p.alpha, mode, w);
-        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_vec, 4, lane);
+        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_maps, 4, lane);
         if (have > 64) {
             finish_words<16>(p.dtype, v + 16, rs, ws + 16, p.alpha, mode, w);
-            store_rows(w, stage, &maps.y, base, x + 64, place0, step, rows, min(have - 64, 64), p.y_vec, 4, lane);
+            store_rows(w, stage, &maps.y, base, x + 64, place0, step, rows, min(have - 64, 64), p.y_maps, 4, lane);
         }
     } else {
         finish_words<32>(p.dtype, v, rs, ws, p.alpha, mode, w);
-        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_vec, 2, lane);
+        store_rows(w, stage, &maps.y, base, x, place0, step, rows, min(have, 64), p.y_maps, 2, lane);
     }
 }
 
 // One persistent block (CG = 1) or pair of blocks (CG = 2, tcgen05.mma.cta_group::2: 256 rows, each block holds its 128 rows and half
 // of the channels) an SM or pair of SMs, over tiles of CG * 128 places x BN channels.  Warp 0 requests the copies, warp 1 issues the
-// MMAs, where places name their rows six warps gather them (each a slot of the ring, so that all are on their way at once), and sixteen
+// MMAs, where places name their rows a warp for every slot of the ring gathers them (so that all are on their way at once; of six such
+// warps the last stands idle where the ring has five slots), and sixteen
 // (tiles of 64 channels: eight) scale, round and store one accumulator while the MMAs fill the other.
 // Large products are bound by the tensor pipe at the clock that the power limit leaves: 8192 x 4096 -> 8192 in 170 us, 3.2 POP/s, 0.98 of
 // twice the measured bf16 rate (its pipe 75 % active by count: operands come in and go to the pipe at 127 of the shared memory's 128
@@ -817,7 +819,7 @@ int launch_tc(tnns_cuda_ctx* ctx, const GemmI8Args& a, cudaStream_t stream) {
     // the weights' tiles hold the swizzle pattern already: plain rows of 128 bytes
     if (CG == 2 && (rc = tnns_tensor_map_2d(&maps.w, 1, a.img, KCH, (unsigned long long)a.experts * a.n_tiles * a.k_tiles * WT, KCH, KCH, BN / CG))) return rc;
     // y by bytes: boxes of 32 rows x 64 bytes
-    if (a.y_vec >= 16) {
+    if (a.y_maps) {
         const int size = tnns_dtype_bytes(a.dtype);
         if ((rc = tnns_tensor_map_2d(&maps.y, 1, a.y, (unsigned long long)a.N * size, (unsigned long long)a.places, (unsigned long long)a.y_stride * size, 64, 32, 64))) return rc;
     }
@@ -872,8 +874,7 @@ int run_product(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w, const int8_t*
     a.y = d_y; a.y_stride = y_stride; a.q_rows = q_rows; a.places = places; a.experts = w->experts; a.N = w->N; a.K = w->K;
     a.n_tiles = w->n_tiles; a.k_tiles = w->k_tiles; a.alpha = alpha;
     a.dtype = dtype; a.status = ctx->d_status;
-    const uintptr_t at = (uintptr_t)d_y | (uintptr_t)(y_stride * tnns_dtype_bytes(dtype));
-    a.y_vec = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
+    a.y_maps = ((uintptr_t)d_y | (uintptr_t)(y_stride * tnns_dtype_bytes(dtype))) % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
     // places an expert has on average, experts that may have one, pieces of 64 channels of those
     const long long rows = ((long long)places + w->experts - 1) / w->experts, met = std::min(w->experts, places);

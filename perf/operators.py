@@ -199,6 +199,8 @@ def prepare(case, seed):
         s["out"] = torch.empty(T, N, dtype=_DT[case["dtype"]], device="cuda")
         if own:
             s["handle"] = _framework()[1].upload_weights_i8(s["w"].data_ptr(), s["w_scale"].data_ptr(), N, K, experts=E)
+            if case["form"] == "down":  # products that are still to be summed keep 32 bits: the sum is what is rounded
+                s["y"] = s["y"].float()
     return s
 
 
@@ -223,10 +225,10 @@ def _run_own(s):
         return s["experts"], s["weights"], s["offsets"], s["rows"], s["slots"]
     up = case["form"] == "up"
     ctx.gemm_i8_experts(s["handle"], s["q"].data_ptr(), s["scale"].data_ptr(), s["rows"].data_ptr() if up else 0, s["offsets"].data_ptr(),
-                        s["y"].data_ptr(), dt, s["q"].shape[0], case["T"] * case["k"], case["alpha"], stream=stream)
+                        s["y"].data_ptr(), dt if up else ft.F32, s["q"].shape[0], case["T"] * case["k"], case["alpha"], stream=stream)
     if up:
         return s["y"]
-    ctx.combine(s["y"].data_ptr(), dt, case["T"] * case["k"], s["slots"].data_ptr(), s["weights"].data_ptr(), case["k"], s["out"].data_ptr(), dt,
+    ctx.combine(s["y"].data_ptr(), ft.F32, case["T"] * case["k"], s["slots"].data_ptr(), s["weights"].data_ptr(), case["k"], s["out"].data_ptr(), dt,
                 case["T"], case["N"], stream=stream)
     return s["out"]
 

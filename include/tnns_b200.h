@@ -500,12 +500,13 @@ enum tnns_dtype { TNNS_F32 = 0, TNNS_F16 = 1, TNNS_BF16 = 2 };
  * or a NaN: scale NaN, q 0, so that the row's products are NaN.  d_x: M rows of K, x_stride elements apart,
  * of type `dtype`; d_q: rows q_stride bytes apart (a multiple of 16, at least K), 16-byte aligned; the bytes
  * between K and q_stride are left as they were.  The same call makes 8-bit weights with a scale for each
- * channel out of N x K floats. */
+ * channel out of N x K floats; an upload takes rows without gaps, so where K is no multiple of 16 the rows are put
+ * together first (cudaMemcpy2D to a pitch of K). */
 int tnns_cuda_quantise_i8(tnns_cuda_ctx* ctx, const void* d_x, int dtype, long long x_stride, int8_t* d_q, long long q_stride,
                           float* d_scale, int M, int K, void* stream);
 
 typedef struct tnns_cuda_weights_i8 tnns_cuda_weights_i8; /* device copy of the 8-bit weights of one layer */
-/* 8-bit weights of `experts` kernels (1: a plain layer; at most 1024), each N x K without gaps, and a scale for each of their
+/* 8-bit weights of `experts` kernels (1: a plain layer; at most 1024), each N x K without gaps (also between rows), and a scale for each of their
  * experts * N channels, both in host or device memory -> the tiles the kernels read (N and K rounded up to 128).
  * K at most 131071: every sum then fits 32 bits.  Synchronises the device.  Done once per layer. */
 int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float* scales, int experts, int N, int K,

@@ -139,8 +139,8 @@ __device__ __forceinline__ uint4 load_piece(const int8_t* row, int k, int K) {
 // such pieces side by side and goes on to others, whose weights it requests before it finishes the present ones.  Bounded by the
 // weights' bytes: a lane (g, t) holds the 32 bytes of pieces 2t and 2t + 1 of channels 2g and 2g + 1 (rows g and g + 8 of the
 // instruction), so a load takes eight whole lines, four instructions multiply a K tile of 2 KB, and no byte passes through shared
-// memory.  The order of K within the tile is the same for weights and rows.  1 x 4096 -> 4096: 5.0 us = 3.4 TB/s, of which the launch and
-// the first bytes' way take 2.4.
+// memory.  The order of K within the tile is the same for weights and rows.  1 x 4096 -> 4096: 5.0 us = 3.4 TB/s (launches
+// back to back, weights from memory), of which the launch and the first bytes' way take 2.4.
 template <int NT, int U>  // U: K tiles whose loads a warp issues together
 __global__ void __launch_bounds__(FEW_WARPS * 32, 2) gemm_i8_few_kernel(const __grid_constant__ GemmI8Args p, int log_s) {
     extern __shared__ int2 s_range[];

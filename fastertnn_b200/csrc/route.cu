@@ -385,7 +385,9 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const T* row, int l
     return c;
 }
 
-// Weights of the chosen, by the full-precision exponential: lane j has slot j.
+// Weights of the chosen, in fp32: lane j has slot j.  The exponential is the library's; a softmax's sum is the one of fast exponentials that
+// the choice made (one more pass over the row for the other would cost as much as the first).  Error against 64 bits over 8191 tokens,
+// 8 of 256: 6e-8, the type's own rounding 3e-8.
 template <typename T>
 __device__ __forceinline__ void finish_token(const RouteArgs& p, const T* row, long long t, int lane, const Choice& c) {
     float s = 0.f;

@@ -392,7 +392,7 @@ __device__ __forceinline__ void store_sums(const CombineArgs& p, long long row, 
 }
 
 // One thread a chunk of VE neighbouring columns (16 bytes of y) of a token, the rows of eight slots on their way at once.  Bounded by
-// memory: every row of y is read once (8192 tokens of 8 x 2048 bf16: 54 us = 5.6 TB/s, 0.86 of the measured copy; rows of 2047: 101 us).  MIS: rows need not start on 16 bytes; the first chunk of a row begins where its results are
+// memory: every row of y is read once (8192 tokens of 8 x 2048 bf16: 50 us = 6.1 TB/s, 0.93 of the measured copy; fp32 92 us = 6.6; rows of 2047: 95 us).  MIS: rows need not start on 16 bytes; the first chunk of a row begins where its results are
 // aligned (at a column up to VE - 1 below 0), and y is fetched as the aligned vectors that hold the chunk.
 template <typename T, bool MIS>
 __global__ void __launch_bounds__(256) combine_kernel(CombineArgs p) {

@@ -485,9 +485,9 @@ int tnns_cuda_conv_noalloc(int type, const int64_t* d_packed_weights, const floa
                            const tnns_shape_t* s, float alpha, int layout, void* stream);
 
 /* ---- Products in 8-bit integers, routing to experts ----------------------------------------
- * The layers of a ternary or binary network that need more than two bits -- its entry and classifier
- * layers, products with outlying channels -- in 8-bit integers with fp32 scales, and the same spread
- * over experts (no reference counterpart).  One layer of experts is
+ * The fully connected layers of a ternary or binary network that need more than two bits -- its classifier,
+ * products with outlying channels -- in 8-bit integers with fp32 scales, and the same spread
+ * over experts (no reference counterpart).  There is no 8-bit convolution: rows come as rows.  One layer of experts is
  *     route -> quantise_i8 -> gemm_i8_experts -> quantise_i8 -> gemm_i8_experts -> combine.
  * All are asynchronous on `stream`, need no workspace, keep nothing from one call
  * for the next, may be captured into a graph, and may run at the same time as other calls of the same
@@ -506,8 +506,9 @@ int tnns_cuda_quantise_i8(tnns_cuda_ctx* ctx, const void* d_x, int dtype, long l
                           float* d_scale, int M, int K, void* stream);
 
 typedef struct tnns_cuda_weights_i8 tnns_cuda_weights_i8; /* device copy of the 8-bit weights of one layer */
-/* 8-bit weights of `experts` kernels (1: a plain layer; at most 1024), each N x K without gaps (also between rows), and a scale for each of their
- * experts * N channels, both in host or device memory -> the tiles the kernels read (N and K rounded up to 128).
+/* 8-bit weights of `experts` kernels (1: a plain layer; at most 1024), each N x K without gaps, between rows neither, and a scale
+ * for each of their experts * N channels, both in host or device memory -> the tiles the kernels read (N and K rounded up to 128, so that an
+ * expert of 64 x 64 takes, and every product reads, four times its bytes).
  * K at most 131071: every sum then fits 32 bits.  Synchronises the device.  Done once per layer. */
 int tnns_cuda_upload_weights_i8(tnns_cuda_ctx* ctx, const int8_t* w, const float* scales, int experts, int N, int K,
                                 tnns_cuda_weights_i8** out);
@@ -535,8 +536,9 @@ typedef struct tnns_route {
 } tnns_route_t;
 /* Experts are ranked by key: the logit where d_bias is NULL, score + bias[expert] otherwise, as 64-bit arithmetic
  * orders them; equal keys go to the lower expert, equal groups to the lower group.  The bias moves the choice only:
- * weights are made of the scores.  An expert whose logit is -inf or NaN, or whose bias is, is never chosen for that
- * token (+inf counts as the largest finite float); slots that find no expert hold expert -1 and weight 0.
+ * weights are made of the scores, in fp32 (a score is off by (100 + |logit|) * 2^-24 of its value at most, with a softmax
+ * the distance from the largest logit in place of |logit|; by about 2^-24 on the average).  An expert whose logit is -inf
+ * or NaN, or whose bias is, is never chosen for that token (+inf counts as the largest finite float); slots that find no expert hold expert -1 and weight 0.
  *   d_logits  T rows of `experts` of type `dtype`, `stride` elements apart
  *   d_experts T x top_k, best first          d_weights  T x top_k floats
  * and, unless all three are NULL, the pairs (token, slot) in the order of their experts, tokens ascending within
@@ -556,7 +558,8 @@ int tnns_cuda_gemm_i8_experts(tnns_cuda_ctx* ctx, const tnns_cuda_weights_i8* w,
                               float alpha, void* stream);
 
 /* out[t] = sum_j d_weights[t][j] * y[d_slots[t][j]] over the top_k slots of token t, j ascending, in fp32, rounded
- * once; slots outside [0, places) are skipped (a token without any gets zeros). */
+ * once; slots outside [0, places) are skipped (a token without any gets zeros).  y in TNNS_F32 keeps the products
+ * unrounded until then; a 16-bit y halves their bytes and rounds every one of them. */
 int tnns_cuda_combine(tnns_cuda_ctx* ctx, const void* d_y, int dtype, long long y_stride, int places, const int32_t* d_slots,
                       const float* d_weights, int top_k, void* d_out, int out_dtype, long long out_stride, int T, int N, void* stream);
 

@@ -537,8 +537,9 @@ typedef struct tnns_route {
 /* Experts are ranked by key: the logit where d_bias is NULL, score + bias[expert] otherwise, as 64-bit arithmetic
  * orders them; equal keys go to the lower expert, equal groups to the lower group.  The bias moves the choice only:
  * weights are made of the scores, in fp32 (a score is off by (100 + |logit|) * 2^-24 of its value at most, with a softmax
- * the distance from the largest logit in place of |logit|; by about 2^-24 on the average; one below 2^-126 may be 0).  An expert whose logit is -inf
- * or NaN, or whose bias is, is never chosen for that token (+inf counts as the largest finite float); slots that find no expert hold expert -1 and weight 0.
+ * the distance from the largest logit in place of |logit|; by about 2^-24 on the average; one below 2^-126 may be 0).
+ * An expert whose logit is -inf or NaN, or whose bias is, is never chosen for that token (+inf counts as the largest
+ * finite float); slots that find no expert hold expert -1 and weight 0.
  *   d_logits  T rows of `experts` of type `dtype`, `stride` elements apart
  *   d_experts T x top_k, best first          d_weights  T x top_k floats
  * and, unless all three are NULL, the pairs (token, slot) in the order of their experts, tokens ascending within
